@@ -39,7 +39,7 @@ EXPORTS = ["fastkv_workspace_bytes", "fastkv_workspace_init", "fastkv_update_kv_
            "fastkv_select_workspace_bytes", "fastkv_compact_f16", "fastkv_compact_ranked_f16", "fastkv_gather_rows", "fastkv_tsp_propagate", "fastkv_head_sum_f16", "fastkv_sp_workspace_bytes", "fastkv_sp_logits_f16", "fastkv_sp_rowmax_f16", "fastkv_sp_rowsum_f16",
            "fastkv_sp_scores_f16", "fastkv_sp_pack_f16", "fastkv_sp_unpack_f16", "fastkv_sp_pick",
            "fastkv_sp_compact_f16", "fastkv_decode_workspace_bytes", "fastkv_decode_append_f16", "fastkv_decode_attention_f16",
-           "fastkv_decode_rmsnorm_f16", "fastkv_decode_rope_f16", "fastkv_decode_silu_mul_f16", "fastkv_decode_greedy_f16", "fastkv_decode_rotary_f16", "fastkv_decode_gemv_f16", "fastkv_update_kv_ptrs_f16", "fastkv_fused_entries_f16", "fastkv_pool_f16", "fastkv_decode_step_attention_f16", "fastkv_debug_contract", "fastkv_debug_mfma16", "fastkv_debug_granule_areas", "fastkv_debug_occupy", "fastkv_debug_fused_placement", "fastkv_placement_violations", "fastkv_set_placement_policy", "fastkv_set_no_wait_mode", "fastkv_set_fused_rolling", "fastkv_no_wait_mode", "fastkv_last_status", "fastkv_profile_enable",
+           "fastkv_decode_rmsnorm_f16", "fastkv_decode_rope_f16", "fastkv_decode_silu_mul_f16", "fastkv_decode_greedy_f16", "fastkv_decode_rotary_f16", "fastkv_decode_gemv_f16", "fastkv_update_kv_ptrs_f16", "fastkv_fused_entries_f16", "fastkv_pool_f16", "fastkv_decode_step_attention_f16", "fastkv_attend_workspace_bytes", "fastkv_window_attention", "fastkv_shared_prefix_attention", "fastkv_decode_penalties", "fastkv_debug_contract", "fastkv_debug_mfma16", "fastkv_debug_granule_areas", "fastkv_debug_occupy", "fastkv_debug_fused_placement", "fastkv_placement_violations", "fastkv_set_placement_policy", "fastkv_set_no_wait_mode", "fastkv_set_fused_rolling", "fastkv_no_wait_mode", "fastkv_last_status", "fastkv_profile_enable",
            "fastkv_profile_kernels", "fastkv_profile_kernel_name", "fastkv_profile_read", "fastkv_strerror", "fastkv_version"]
 
 _lib = None
@@ -129,6 +129,15 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
     L.fastkv_pool_f16.restype = ci
     L.fastkv_decode_gemv_f16.argtypes = [ci, ci, vp, i64, vp, ctypes.c_float, ci, ctypes.POINTER(vp), ctypes.POINTER(ci), ci, vp, i64, vp, i64, vp]
     L.fastkv_decode_gemv_f16.restype = ci
+    L.fastkv_attend_workspace_bytes.argtypes = [ci] * 10
+    L.fastkv_attend_workspace_bytes.restype = sz
+    L.fastkv_window_attention.argtypes = [ci] * 6 + [vp, i64p, vp, i64p, vp, i64p, ci, vp, ci, ci, ci, ci, ctypes.c_float, vp, vp, sz, vp]
+    L.fastkv_window_attention.restype = ci
+    L.fastkv_shared_prefix_attention.argtypes = [ci] * 6 + [vp, i64p, vp, i64p, vp, i64p, ci, vp, i64p, vp, i64p, ci, vp, ci, ci, ctypes.c_float,
+                                                            vp, vp, sz, vp]
+    L.fastkv_shared_prefix_attention.restype = ci
+    L.fastkv_decode_penalties.argtypes = [ci, ci, ci, vp, i64, vp, i64, ci] + [vp, ci] * 5 + [vp, i64, vp, i64, vp, i64, vp]
+    L.fastkv_decode_penalties.restype = ci
     L.fastkv_debug_occupy.argtypes = [ci, ci, i64, vp]
     L.fastkv_debug_occupy.restype = ci
     L.fastkv_debug_fused_placement.argtypes = [ci, vp, ctypes.c_size_t]

@@ -48,6 +48,10 @@ extern "C" {
 #define FASTKV_ORDER_SCORE 1 /* score descending, ties by ascending position: the order of  */
                              /* `topk(sorted=True)` (utils.py:113) with a canonical tie rule */
 
+#define FASTKV_F16 0 /* element types of the entry points that take a `dtype` */
+#define FASTKV_BF16 1
+#define FASTKV_F32 2 /* logits only */
+
 /* Problem description shared by the entry points (plain data, passed by pointer). */
 typedef struct fastkv_problem {
     int32_t B;         /* batch */
@@ -431,6 +435,50 @@ int fastkv_decode_greedy_f16(int32_t B, int32_t V, const void *logits, int64_t r
 int fastkv_decode_gemv_f16(int32_t B, int32_t K, const void *x, int64_t x_row_stride, const void *norm_weight, float eps,
                            int32_t n_mats, const void *const *weights, const int32_t *rows, int32_t glu, const void *residual,
                            int64_t res_row_stride, void *out, int64_t out_row_stride, void *stream);
+
+/*
+ * ---- Attention forms over a cache (csrc/attend.hip) ----
+ * A call has T >= 1 new tokens per request; their K / V rows are already in the cache (rows len .. len + T - 1).  Query t of request b
+ * stands at position p = len[b] + t; H / Hkv query heads share a KV head (any whole ratio).  out [B,T,H*D] contiguous, of the inputs'
+ * type = sum softmax(scaling q.k) v over the rows it sees, fp32 sums; p < 0 (an idle request, left padding): zeros.
+ *   fastkv_window_attention          rows j <= p of the request's cache with j < sinks or j > p - window (window 0: all j <= p)
+ *   fastkv_shared_prefix_attention   all prefix_rows rows of ONE prefix [Hkv,prefix_rows,D] that every request continues, and the
+ *                                    request's own rows j <= p.  The prefix is read once for the batch, not once per request
+ * dtype FASTKV_F16 | FASTKV_BF16; D 64, 128 or 256; element strides q {batch, head, token}, k / v {batch, head, row}, prefix {head, row}:
+ * all multiples of 8, head-dim stride 1, 16-byte aligned bases.  rows: rows of the cache per request.  len_dev: int32 on the device,
+ * one per request (len_step 1) or one for all (0); a length above rows - T counts as rows - T; NULL (window only): rows - T for all.
+ * advance != 0: len_dev grows by T behind the call (not where it is negative; a full cache is reported as FASTKV_EOVERFLOW, as by
+ * fastkv_decode_attention_f16).  K / V rows that nothing sees may hold anything, infinities and NaN included.  scaling > 0.
+ * workspace: fastkv_attend_workspace_bytes (0: none needed; prefix 0 for the window form), 16-byte aligned, nothing to initialise and
+ * nothing kept in it between calls.  Sums are added in a fixed order: the same call gives the same bits.
+ */
+size_t fastkv_attend_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t T, int32_t rows, int32_t window, int32_t sinks,
+                                     int32_t prefix, int32_t advance);
+int fastkv_window_attention(int32_t dtype, int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t T, const void *q, const int64_t q_strides[3],
+                            const void *k, const int64_t k_strides[3], const void *v, const int64_t v_strides[3], int32_t rows,
+                            int32_t *len_dev, int32_t len_step, int32_t advance, int32_t window, int32_t sinks, float scaling, void *out,
+                            void *workspace, size_t workspace_bytes, void *stream);
+int fastkv_shared_prefix_attention(int32_t dtype, int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t T, const void *q, const int64_t q_strides[3],
+                                   const void *k_prefix, const int64_t kp_strides[2], const void *v_prefix, const int64_t vp_strides[2],
+                                   int32_t prefix_rows, const void *k, const int64_t k_strides[3], const void *v, const int64_t v_strides[3],
+                                   int32_t rows, int32_t *len_dev, int32_t len_step, int32_t advance, float scaling, void *out, void *workspace,
+                                   size_t workspace_bytes, void *stream);
+
+/*
+ * Penalties, biases and masks on a step's logits in ONE launch (csrc/penalties.hip), in front of fastkv_decode_greedy_f16 or a sampler.
+ * Row b, token v, in fp32 and in this order, rounded once to `dtype` (FASTKV_F16 | FASTKV_BF16 | FASTKV_F32):
+ *   v among tokens[b, :n_tokens[b]]: x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *   c = how often among tokens[b, n_prompt[b]:n_tokens[b]]:  x -= frequency[b] * c;  c > 0: x -= presence[b]
+ *   x += bias[b, v];  bit v % 32 of allowed[b, v / 32] clear: x = -inf
+ * tokens int64 [B,L] (ids outside [0,V) count for nothing), n_tokens / n_prompt int32, the three penalties fp32, all on the device;
+ * `*_step` 1: one value per row, 0: one for all; NULL: L / 0 / that penalty is not applied.  bias fp32, allowed uint32 words: row
+ * stride 0 = one row for all, NULL: none.  Strides in elements.  out may be `logits` itself with the same stride, and may not overlap it otherwise.
+ */
+int fastkv_decode_penalties(int32_t dtype, int32_t B, int32_t V, const void *logits, int64_t row_stride, const int64_t *tokens,
+                            int64_t token_stride, int32_t L, const int32_t *n_tokens, int32_t n_tokens_step, const int32_t *n_prompt,
+                            int32_t n_prompt_step, const float *repetition, int32_t repetition_step, const float *presence,
+                            int32_t presence_step, const float *frequency, int32_t frequency_step, const float *bias,
+                            int64_t bias_stride, const int32_t *allowed, int64_t allowed_stride, void *out, int64_t out_stride, void *stream);
 
 /*
  * Test hook (not part of the operator): evaluates primitive `op` of the arithmetic contract element-wise
