@@ -60,6 +60,7 @@ struct AttendArgs {
     int slots;                               // slices per row; 0: the result goes to `out`
     int packed_tiles, packed_split, slot0;   // shared prefix, few rows per request: row tiles over ALL requests in front of the grid
     int tiles, split;                        // row tiles per request, key slices
+    bool near_rows;
 };
 
 template <bool BF> __device__ __forceinline__ att_f16 att_mfma(att_u4 a, att_u4 b, att_f16 c)
@@ -117,44 +118,124 @@ struct AttKeys {                             // the keys of one item, and which 
     int64_t k0_r, v0_r, k_r, v_r;
     int n0, lo, N;                           // segment 0; first row of segment 1; all
     int window, sinks;
-    __device__ __forceinline__ bool sees(int u, int p) const
+    bool near_rows;                          // 64 rows of any of the four lie within 31 bits of bytes
+};
+
+// Which keys a row at position p >= 0 sees, by their number from u0 on: k < end, and k < first (segment 0 and sinks) or k > before (the window).
+// Written without branches: a select per score (a masked store under a branch has cost wrong code here).
+struct AttSees {
+    int end, first, before;
+    __device__ __forceinline__ AttSees(const AttKeys &K, int u0, int p)
     {
-        const int j = lo + u - n0;
-        return u < N && (u < n0 || (j <= p && (j > p - window || j < sinks)));
+        const int o = K.n0 - K.lo;                           // row j is key j + o
+        end = min(K.N, p + o + 1) - u0;
+        first = max(K.n0, K.sinks + o) - u0;
+        before = p - K.window + o - u0;
     }
+    __device__ __forceinline__ bool operator()(int k) const { return (k < end) & ((k < first) | (k > before)); }
 };
 
 struct AttState { float m, l; };
 
-// One tile of 32*NB keys, u0 .. : `ks`, `vs` the tile in shared memory; Q the wave's 32 query rows; `edge`: some row may not see some
-// key of the tile; `wild`: keys of the tile (bits) whose V row holds an infinity or NaN, given for edge tiles only -- a row that does not see
-// such a key must not be touched by it (0 * inf), so these keys are taken out of the product and added for the rows that see them.
-template <int D, bool BF, int NB>
-__device__ __forceinline__ void att_tile(const uint16_t *ks, const uint16_t *vs, const att_u4 (&Q)[D / 16], att_f16 (&O)[D / 32], AttState &st,
-                                         float c, const AttKeys &K, int u0, int p, bool edge, uint64_t wild)
-{
-    const int lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
-    att_f16 S[NB];
+// Rows u0 .. u0 + 32*NB - 1 of K and V on their way to shared memory, brought by NW waves without passing registers (the 16 bytes of lane l
+// land at a wave's base + 16 l; the swizzle is in which piece of the row the lane asks for).
+template <int D, int NB, int NW> struct AttLoad {
+    static constexpr int KT = 32 * NB, C = D / 8, RPI = 64 / C, CH = KT / (RPI * NW);     // rows per instruction, instructions per wave
+    static constexpr int NV = RPI * NW >= 8 ? 1 : 8 / (RPI * NW);                         // distinct swizzles over a lane's rows
+    typedef __attribute__((address_space(3))) uint32_t lds_u32;
+    typedef __attribute__((address_space(1))) uint32_t glb_u32;
+
+    static __device__ __forceinline__ int row_of(int i, int w, int lane) { return (i * NW + w) * RPI + lane / C; }
+    static __device__ __forceinline__ bool plain(const AttKeys &K, int u0) { return K.near_rows && u0 + KT <= K.N && (u0 + KT <= K.n0 || u0 >= K.n0); }
+
+    // Whole tiles of one segment: buffer loads, a 32-bit offset per lane and the tile's base in scalar registers.  Others (the tile over
+    // the segments' seam, the last one, rows further apart than 32 bits reach): an address per lane, and zeros behind the last key -- their
+    // scores are cut off, but a V row there must be finite.
+    static __device__ __forceinline__ void issue(const AttKeys &K, int u0, bool value, uint16_t *dst, int w)
+    {
+        const int lane = threadIdx.x & 63;
+        const bool first = u0 + KT <= K.n0;
+        if (plain(K, u0)) {
+            const int64_t r = value ? (first ? K.v0_r : K.v_r) : (first ? K.k0_r : K.k_r);
+            const uint16_t *base = (value ? (first ? K.v0 : K.v) : (first ? K.k0 : K.k)) + (first ? u0 : K.lo + u0 - K.n0) * r;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(base), 0, 0x7fffffff, 0x00020000);
+            const int step = (int)r * 2;
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb) {
+            for (int i = 0; i < CH; ++i) {
+                const int c = (lane % C) ^ att_swz(row_of(i % NV, w, lane));
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_u32 *)(dst + (i * NW + w) * RPI * D), 16, lane / C * step + c * 16,
+                                                         (i * NW + w) * RPI * step, 0, 0);
+            }
+        } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) S[kb][r] = 0.0f;
-    }
-    const int swk = att_swz(col);
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-#pragma unroll
-        for (int kb = 0; kb < NB; ++kb) {
-            const att_u4 a = *reinterpret_cast<const att_u4 *>(ks + (kb * 32 + col) * D + ((2 * s + hi) ^ swk) * 8);
-            S[kb] = att_mfma<BF>(a, Q[s], S[kb]);
+            for (int i = 0; i < CH; ++i) {
+                const int row = row_of(i, w, lane), u = u0 + row, c = (lane % C) ^ att_swz(row);
+                if (u < K.N) {
+                    const bool f = u < K.n0;
+                    const int64_t j = f ? u : K.lo + u - K.n0;
+                    const uint16_t *src = (value ? (f ? K.v0 : K.v) + j * (f ? K.v0_r : K.v_r) : (f ? K.k0 : K.k) + j * (f ? K.k0_r : K.k_r)) + c * 8;
+                    __builtin_amdgcn_global_load_lds((const glb_u32 *)src, (lds_u32 *)(dst + (i * NW + w) * RPI * D), 16, 0, 0);
+                } else {
+                    *reinterpret_cast<att_u4 *>(dst + (i * NW + w) * RPI * D + lane * 8) = att_u4{0, 0, 0, 0};
+                }
+            }
         }
     }
+    // this lane's V pieces, landed: which rows hold an infinity or NaN
+    template <bool BF> static __device__ __forceinline__ void scan(const uint16_t *vs, int w, unsigned long long *wild)
+    {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const att_u4 x = *reinterpret_cast<const att_u4 *>(vs + (i * NW + w) * RPI * D + lane * 8);
+            if (att_wild<BF>(x[0]) || att_wild<BF>(x[1]) || att_wild<BF>(x[2]) || att_wild<BF>(x[3])) atomicOr(wild, 1ull << row_of(i, w, lane));
+        }
+    }
+};
+
+// all of this wave's loads to shared memory but the last LEFT have landed (they come back in order)
+template <int LEFT> __device__ __forceinline__ void att_landed()
+{
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (LEFT & 15) | (LEFT >> 4) << 14);
+    asm volatile("" ::: "memory");
+}
+// this wave's reads of shared memory are done: what they read may be overwritten
+__device__ __forceinline__ void att_read_done()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
+// S^T = K Q^T of a tile of 32*NB keys
+template <int D, bool BF, int NB> __device__ __forceinline__ void att_scores(const uint16_t *ks, const att_u4 (&Q)[D / 16], att_f16 (&S)[NB])
+{
+    const int lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5, sw = att_swz(col);
+    const uint16_t *at[4];                   // piece (2 s + hi) ^ sw of row col: the swizzle is in the low three bits
+#pragma unroll
+    for (int x = 0; x < 4; ++x) at[x] = ks + col * D + ((2 * x + hi) ^ sw) * 8;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[kb][r] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb) S[kb] = att_mfma<BF>(*reinterpret_cast<const att_u4 *>(at[s & 3] + (s >> 2) * 64 + kb * 32 * D), Q[s], S[kb]);
+}
+
+// the running softmax over a tile's scores, u0 its first key; `edge`: some row may not see some key.  P^T comes out as the second operand of V^T P^T.
+template <int D, bool BF, int NB>
+__device__ __forceinline__ void att_softmax(att_f16 (&S)[NB], att_u4 (&P)[NB * 2], att_f16 (&O)[D / 32], AttState &st, float c, const AttKeys &K, int u0,
+                                            int p, bool edge)
+{
+    const int hi = threadIdx.x >> 5 & 1;
     if (edge) {
+        const AttSees sees(K, u0 + 4 * hi, p);
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (!K.sees(u0 + kb * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi, p)) S[kb][r] = -INFINITY;
+            for (int r = 0; r < 16; ++r) S[kb][r] = sees(kb * 32 + (r & 3) + 8 * (r >> 2)) ? S[kb][r] : -INFINITY;
     }
     float tm = -INFINITY;
 #pragma unroll
@@ -173,7 +254,6 @@ __device__ __forceinline__ void att_tile(const uint16_t *ks, const uint16_t *vs,
             for (int r = 0; r < 16; ++r) O[db][r] *= f;
     }
     const float mc = (st.m == -INFINITY ? 0.0f : st.m * c) - (BF ? 0.0f : ATT_LIFT);
-    att_u4 P[NB * 2];
     float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
@@ -185,85 +265,59 @@ __device__ __forceinline__ void att_tile(const uint16_t *ks, const uint16_t *vs,
             P[kb * 2 + (r >> 3)][(r & 7) >> 1] = att_pack<BF>(a, b);
         }
     st.l += l0 + l1;
+}
+
+// O^T += V^T P^T.  `wild`: keys of the tile (bits) whose V row holds an infinity or NaN, given where some row does not see some key -- a row
+// must not be touched by a key that it does not see (0 * inf), so these keys are taken out of the product and added for the rows that see them.
+template <int D, bool BF, int NB>
+__device__ __forceinline__ void att_values(const uint16_t *vs, const att_u4 (&P)[NB * 2], att_f16 (&O)[D / 32], const AttKeys &K, int u0, int p,
+                                           uint64_t wild)
+{
     // lane i of a group of 16 addresses row i / 4, elements 4 * (i % 4) of a 4 x 16 block and receives column i
-    const int gi = lane & 15, dsub = (lane >> 4 & 1) * 16 + (gi & 3) * 4, krow = gi >> 2;
+    const int lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5, gi = lane & 15, krow = gi >> 2;
+    const int piece = (lane >> 4 & 1) * 2 + (gi >> 1 & 1), sw = att_swz(4 * hi + krow);
+    typedef __attribute__((address_space(3))) att_s4 lds_s4;
+    const uint16_t *at[2];                   // dims 32 db + 8 piece + ..: the swizzle is in the low three bits of 4 db + piece
+#pragma unroll
+    for (int x = 0; x < 2; ++x) at[x] = vs + (4 * hi + krow) * D + ((4 * x + piece) ^ sw) * 8 + (gi & 1) * 4;
 #pragma unroll
     for (int s = 0; s < NB * 2; ++s) {
-        const int r0 = s * 16 + 4 * hi + krow, r1 = r0 + 8;
-        const uint16_t *v0 = vs + r0 * D, *v1 = vs + r1 * D;
-        const int w0 = att_swz(r0), w1 = att_swz(r1);
-        const uint32_t cut = edge ? (uint32_t)(wild >> (s * 16 + 4 * hi)) : 0u;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) {
-            const int d = db * 32 + dsub;
-            typedef __attribute__((address_space(3))) att_s4 lds_s4;
-            const att_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(v0 + ((d >> 3) ^ w0) * 8 + (d & 7)));
-            const att_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(v1 + ((d >> 3) ^ w1) * 8 + (d & 7)));
+            const uint16_t *v = at[db & 1] + (db >> 1) * 64 + s * 16 * D;
+            const att_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)v);
+            const att_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(v + 8 * D));
             const uint2 xa = __builtin_bit_cast(uint2, x), ya = __builtin_bit_cast(uint2, y);
             att_u4 a = {xa.x, xa.y, ya.x, ya.y};
-            if (edge && wild) {
-                const uint32_t b = (cut & 0xfu) | (cut >> 4 & 0xf0u);
+            if (wild) {
+                const uint32_t cut = (uint32_t)(wild >> (s * 16 + 4 * hi)), b = (cut & 0xfu) | (cut >> 4 & 0xf0u);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) a[e] &= (b >> (2 * e) & 1 ? 0u : 0xffffu) | (b >> (2 * e + 1) & 1 ? 0u : 0xffff0000u);
             }
             O[db] = att_mfma<BF>(a, P[s], O[db]);
         }
     }
-    if (edge && wild) {
-        for (uint64_t left = wild; left; left &= left - 1) {
-            const int key = __builtin_ctzll(left);
-            uint32_t w = 0;
+    for (uint64_t left = wild; left; left &= left - 1) {
+        const int key = __builtin_ctzll(left);
+        uint32_t w = 0;
 #pragma unroll
-            for (int s = 0; s < NB * 2; ++s)
+        for (int s = 0; s < NB * 2; ++s)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)      // the word of P that holds keys (2e & 3) + 8 (e >> 1) + 4 hi (+1) of step s
-                    w = s * 16 + (e >> 1) * 8 + (e & 1) * 2 == (key & ~5) ? P[s][e] : w;
-            w = (uint32_t)__shfl((int)w, col + 32 * (key >> 2 & 1), 64);
-            const float pk = att_float<BF>(key & 1 ? w >> 16 : w & 0xffffu);
-            const bool seen = K.sees(u0 + key, p);
+            for (int e = 0; e < 4; ++e)          // the word of P that holds keys (2e & 3) + 8 (e >> 1) + 4 hi (+1) of step s
+                w = s * 16 + (e >> 1) * 8 + (e & 1) * 2 == (key & ~5) ? P[s][e] : w;
+        w = (uint32_t)__shfl((int)w, col + 32 * (key >> 2 & 1), 64);
+        const float pk = att_float<BF>(key & 1 ? w >> 16 : w & 0xffffu);
+        const bool seen = AttSees(K, u0, p)(key);
 #pragma unroll
-            for (int db = 0; db < D / 32; ++db)
+        for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = db * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi;
-                    const float x = att_float<BF>(vs[key * D + ((d >> 3) ^ att_swz(key)) * 8 + (d & 7)]);
-                    if (seen) O[db][r] = __builtin_fmaf(pk, x, O[db][r]);
-                }
-        }
+            for (int r = 0; r < 16; ++r) {
+                const int d = db * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi;
+                const float x = att_float<BF>(vs[key * D + ((d >> 3) ^ att_swz(key)) * 8 + (d & 7)]);
+                O[db][r] = seen ? __builtin_fmaf(pk, x, O[db][r]) : O[db][r];
+            }
     }
 }
-
-// Registers of a tile on its way to shared memory: NT threads, 32*NB rows of K and V, CH pieces each per thread
-template <int D, int NB, int NT> struct AttStage {
-    static constexpr int C = D / 8, CH = 32 * NB * C / NT;
-    att_u4 k[CH], v[CH];
-    __device__ __forceinline__ void fetch(const AttKeys &K, int u0, int tid)
-    {
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int id = i * NT + tid, u = u0 + id / C, e = id % C * 8;
-            const att_u4 z = {0, 0, 0, 0};
-            k[i] = v[i] = z;                 // behind the last key: zeros (their scores are cut off, their V rows must be finite)
-            if (u < K.N) {
-                const bool first = u < K.n0;
-                const int64_t j = first ? u : K.lo + u - K.n0;
-                k[i] = *reinterpret_cast<const att_u4 *>((first ? K.k0 : K.k) + j * (first ? K.k0_r : K.k_r) + e);
-                v[i] = *reinterpret_cast<const att_u4 *>((first ? K.v0 : K.v) + j * (first ? K.v0_r : K.v_r) + e);
-            }
-        }
-    }
-    template <bool BF> __device__ __forceinline__ void commit(uint16_t *ks, uint16_t *vs, int tid, bool edge, unsigned long long *wild)
-    {
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int id = i * NT + tid, row = id / C, c = (id % C) ^ att_swz(row);
-            *reinterpret_cast<att_u4 *>(ks + row * D + c * 8) = k[i];
-            *reinterpret_cast<att_u4 *>(vs + row * D + c * 8) = v[i];
-            if (edge && (att_wild<BF>(v[i][0]) || att_wild<BF>(v[i][1]) || att_wild<BF>(v[i][2]) || att_wild<BF>(v[i][3])))
-                atomicOr(wild, 1ull << row);
-        }
-    }
-};
 
 __device__ __forceinline__ int att_len(const AttendArgs &A, int b)
 {
@@ -282,7 +336,7 @@ __device__ __forceinline__ int att_spread(int i, int n)
     return i < full ? (i & 7) * per + (i >> 3) : i;
 }
 
-template <int RW> __device__ __forceinline__ AttItem att_item(const AttendArgs &A)
+template <int RWP, int RW> __device__ __forceinline__ AttItem att_item(const AttendArgs &A)
 {
     AttItem it;
     int i = blockIdx.x;
@@ -290,7 +344,7 @@ template <int RW> __device__ __forceinline__ AttItem att_item(const AttendArgs &
     it.packed = i < np;
     if (it.packed) {                                         // (tile fastest: the tiles of one slice share its keys)
         i = att_spread(i, np);
-        it.row0 = i % A.packed_tiles * (32 * RW);
+        it.row0 = i % A.packed_tiles * (32 * RWP);
         i /= A.packed_tiles;
         it.slice = i % A.packed_split;
         it.hk = i / A.packed_split;
@@ -310,18 +364,13 @@ template <int RW> __device__ __forceinline__ AttItem att_item(const AttendArgs &
     return it;
 }
 
-// RW = 4: rows, RW = 1: keys (see above)
-template <int D, bool BF, int RW>
-__global__ void __launch_bounds__(ATT_THREADS) attend_kernel(const AttendArgs A)
+// an item, by four waves.  RW = 4: rows, RW = 1: keys (see above)
+template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(const AttendArgs &A, const AttItem &it, uint16_t *smem)
 {
     constexpr int NB = RW == 4 ? 2 : 1, KT = 32 * NB, KW = 4 / RW;
     constexpr int TILE = KT * D;                             // elements of a K (or V) tile
-    constexpr int NBUF = RW == 4 ? 2 : 4;                    // two tiles of the workgroup | one tile of each wave
-    __shared__ __attribute__((aligned(16))) uint16_t smem[NBUF * 2 * TILE];
-    __shared__ unsigned long long s_wild[RW == 4 ? 3 : 4];
-    __shared__ float s_ml[KW][32][2];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 31, hi = lane >> 5;
-    const AttItem it = att_item<RW>(A);
+    __shared__ unsigned long long s_wild[4];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hi = lane >> 5;
     const int TG = A.T * A.G, R = it.packed ? A.B * TG : TG;
     // ---- this lane's query row
     const int wrow0 = it.row0 + (RW == 4 ? w * 32 : 0);
@@ -338,164 +387,202 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_kernel(const AttendArgs A)
     }
     // ---- the item's keys
     AttKeys K;
-    int p_lo = 0, p_hi = 0;                                  // positions of this wave's rows
-    int u_lo, u_hi;                                          // this workgroup's share of them
+    int p_lo = 0, p_hi = 0, e_lo = 0, e_hi = 0;              // positions of this wave's rows, of the workgroup's
+    K.near_rows = A.near_rows;
+    K.k0_r = A.k0_r;
+    K.v0_r = A.v0_r;
+    K.k_r = A.k_r;
+    K.v_r = A.v_r;
+    K.window = A.window;
+    K.sinks = A.sinks;
     if (it.packed) {
         K.n0 = K.N = A.prefix;
         K.lo = 0;
-        K.window = K.sinks = 0;
         K.k = K.v = nullptr;
-        K.k_r = K.v_r = 0;
         K.k0 = A.k0 + it.hk * A.k0_h;
         K.v0 = A.v0 + it.hk * A.v0_h;
     } else {
-        const int last = min(it.row0 + 32 * RW, R) - 1;
-        const int pa = n + it.row0 / A.G, pb = n + last / A.G;                 // positions of the workgroup's rows
-        K.window = A.window;
-        K.sinks = A.sinks;
-        K.lo = max(0, pa - A.window + 1);
+        const int n_ = att_len(A, it.b);                     // (uniform: this and what follows is scalar)
+        e_lo = n_ + it.row0 / A.G;
+        e_hi = n_ + (min(it.row0 + 32 * RW, R) - 1) / A.G;
+        p_lo = n_ + wrow0 / A.G;
+        p_hi = n_ + (min(wrow0 + 32, R) - 1) / A.G;
+        K.lo = max(0, e_lo - A.window + 1);
         K.n0 = A.packed_tiles ? 0 : A.prefix ? A.prefix : min(A.sinks, K.lo);
-        if (pb < 0) K.n0 = K.lo = 0;                         // rows that see nothing
-        K.N = K.n0 + max(0, pb + 1 - K.lo);
+        if (e_hi < 0) K.n0 = K.lo = 0;                       // rows that see nothing
+        K.N = K.n0 + max(0, e_hi + 1 - K.lo);
         K.k0 = A.k0 + it.b * A.k0_b + it.hk * A.k0_h;
         K.v0 = A.v0 + it.b * A.v0_b + it.hk * A.v0_h;
         K.k = A.k + it.b * A.k_b + it.hk * A.k_h;
         K.v = A.v + it.b * A.v_b + it.hk * A.v_h;
-        K.k_r = A.k_r;
-        K.v_r = A.v_r;
-        p_lo = n + wrow0 / A.G;
-        p_hi = n + (min(wrow0 + 32, R) - 1) / A.G;
     }
-    K.k0_r = A.k0_r;
-    K.v0_r = A.v0_r;
-    const int nsl = it.packed ? A.packed_split : A.split;
+    int u_lo;                                                // this workgroup's share of the keys: u_lo .. K.N - 1
     {
+        const int nsl = it.packed ? A.packed_split : A.split;
         const int all = (K.N + KT * KW - 1) / (KT * KW), per = (all + nsl - 1) / nsl;
         u_lo = min(K.N, it.slice * per * KT * KW);
-        u_hi = min(K.N, u_lo + per * KT * KW);
-        K.N = u_hi;                                          // keys behind the share are no keys
+        K.N = min(K.N, u_lo + per * KT * KW);
     }
-    // what a tile at u needs of this wave (positions of its rows: p_lo .. p_hi)
-    auto edge_at = [&](int u, int a, int z) {                // rows at positions a .. z: not every row sees every key
-        if (u + KT > K.N) return true;
+    // rows at positions a .. z: some of them does not see some key in the tile at u (keys behind the last one aside)
+    auto mixed = [&](int u, int a, int z) {
         if (u + KT <= K.n0) return false;
-        if (u < K.n0) return true;
-        const int j = K.lo + u - K.n0;
-        return j + KT - 1 > a || j <= z - K.window;
+        const int j = K.lo + max(u, K.n0) - K.n0, j1 = K.lo + min(u + KT, K.N) - K.n0;
+        return j1 - 1 > a || j <= z - K.window;
     };
-    const bool idle_wave = wrow0 >= R;
-    const int e_lo = RW == 4 && !it.packed ? n + it.row0 / A.G : p_lo, e_hi = RW == 4 && !it.packed ? n + (min(it.row0 + 32 * RW, R) - 1) / A.G : p_hi;
     AttState st = {-INFINITY, 0.0f};
-    att_f16 O[D / 32];
+    att_f16 O[D / 32], S[NB];
+    att_u4 P[NB * 2];
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
         for (int e = 0; e < 16; ++e) O[db][e] = 0.0f;
 
     if (RW == 4) {
-        AttStage<D, NB, ATT_THREADS> sg;
+        typedef AttLoad<D, NB, 4> Load;
         if (tid < 3) s_wild[tid] = 0;
-        __syncthreads();
-        const int nt = (u_hi - u_lo + KT - 1) / KT;
+        const int nt = (K.N - u_lo + KT - 1) / KT;
         if (nt > 0) {
-            sg.fetch(K, u_lo, tid);
-            sg.template commit<BF>(smem, smem + TILE, tid, edge_at(u_lo, e_lo, e_hi), &s_wild[0]);
+            Load::issue(K, u_lo, false, smem, w);
+            Load::issue(K, u_lo, true, smem + TILE, w);
         }
+        att_landed<0>();
+        __syncthreads();
+        if (nt > 0 && mixed(u_lo, e_lo, e_hi)) Load::template scan<BF>(smem + TILE, w, &s_wild[0]);
         __syncthreads();
         for (int i = 0; i < nt; ++i) {
-            const int u = u_lo + i * KT, cur = i & 1;
-            if (i + 1 < nt) sg.fetch(K, u + KT, tid);
-            bool skip = idle_wave;
-            if (!it.packed && u >= K.n0) {                    // a tile that none of this wave's rows sees
+            const int u = u_lo + i * KT;
+            uint16_t *cur = smem + (i & 1) * 2 * TILE, *nxt = smem + (i & 1 ^ 1) * 2 * TILE;
+            if (i + 1 < nt) {                                 // (the other buffer was last read before the barrier)
+                Load::issue(K, u + KT, false, nxt, w);
+                Load::issue(K, u + KT, true, nxt + TILE, w);
+            }
+            bool skip = wrow0 >= R;                           // no rows, or a tile that none of them sees
+            if (!it.packed && u >= K.n0) {
                 const int j = K.lo + u - K.n0;
                 skip = skip || j > p_hi || (j + KT - 1 <= p_lo - K.window && j >= K.sinks);
             }
-            if (!skip)
-                att_tile<D, BF, NB>(smem + cur * 2 * TILE, smem + cur * 2 * TILE + TILE, Q, O, st, A.c, K, u, p, edge_at(u, p_lo, p_hi),
-                                    s_wild[i % 3]);
-            if (i + 1 < nt)
-                sg.template commit<BF>(smem + (cur ^ 1) * 2 * TILE, smem + (cur ^ 1) * 2 * TILE + TILE, tid, edge_at(u + KT, e_lo, e_hi),
-                                       &s_wild[(i + 1) % 3]);
+            if (!skip) {
+                const bool mx = mixed(u, p_lo, p_hi);
+                att_scores<D, BF, NB>(cur, Q, S);
+                att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, mx || u + KT > K.N);
+                att_values<D, BF, NB>(cur + TILE, P, O, K, u, p, mx ? s_wild[i % 3] : 0);
+            }
+            att_landed<0>();
+            if (i + 1 < nt && mixed(u + KT, e_lo, e_hi)) Load::template scan<BF>(nxt + TILE, w, &s_wild[(i + 1) % 3]);
             if (tid == 0) s_wild[(i + 2) % 3] = 0;           // last read a tile ago, written a tile from now
             __syncthreads();
         }
     } else {
-        AttStage<D, NB, 64> sg;
+        typedef AttLoad<D, NB, 1> Load;
         uint16_t *ks = smem + w * 2 * TILE, *vs = ks + TILE;
         int u = u_lo + w * KT;
-        if (u < u_hi) sg.fetch(K, u, lane);
-        for (; u < u_hi; u += KT * KW) {
-            const bool edge = edge_at(u, p_lo, p_hi);
-            if (lane == 0) s_wild[w] = 0;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            sg.template commit<BF>(ks, vs, lane, edge, &s_wild[w]);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if (u + KT * KW < u_hi) sg.fetch(K, u + KT * KW, lane);
-            att_tile<D, BF, NB>(ks, vs, Q, O, st, A.c, K, u, p, edge, s_wild[w]);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+        if (u < K.N) {
+            Load::issue(K, u, false, ks, 0);
+            Load::issue(K, u, true, vs, 0);
+        }
+        for (; u < K.N; u += KT * KW) {
+            const int un = u + KT * KW;
+            const bool more = un < K.N;
+            if (Load::plain(K, u)) att_landed<Load::CH>();
+            else att_landed<0>();
+            att_scores<D, BF, NB>(ks, Q, S);
+            att_read_done();
+            if (more) Load::issue(K, un, false, ks, 0);
+            const bool mx = mixed(u, p_lo, p_hi);
+            att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, mx || u + KT > K.N);
+            if (more && Load::plain(K, un)) att_landed<Load::CH>();
+            else att_landed<0>();
+            uint64_t wild = 0;
+            if (mx) {
+                if (lane == 0) s_wild[w] = 0;
+                asm volatile("" ::: "memory");
+                Load::template scan<BF>(vs, 0, &s_wild[w]);  // (one wave's accesses to shared memory are in order)
+                asm volatile("" ::: "memory");
+                wild = s_wild[w];
+            }
+            att_values<D, BF, NB>(vs, P, O, K, u, p, wild);
+            att_read_done();
+            if (more) Load::issue(K, un, true, vs, 0);
         }
     }
     st.l = att_other_half_sum(st.l);
 
-    // ---- the waves' states over their keys, joined
-    if (KW > 1) {
-        if (hi == 0) { s_ml[w][col][0] = st.m; s_ml[w][col][1] = st.l; }
-        __syncthreads();                                     // (also: nobody reads tiles any more)
-        float M = -INFINITY;
+    if (RW == 4) {
+        if (r >= R) return;
+        if (A.slots) {
+            const int64_t row = ((int64_t)b * A.H + h) * A.T + t;
+            float *ml = A.part_ml + (row * A.slots + it.slot) * 2, *o = A.part_o + (row * A.slots + it.slot) * D;
+            if (hi == 0) { ml[0] = st.m; ml[1] = p < 0 ? -1.0f : st.l; }           // -1: the row sees nothing
 #pragma unroll
-        for (int i = 0; i < KW; ++i) M = fmaxf(M, s_ml[i][col][0]);
-        float L = 0.0f;
+            for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-        for (int i = 0; i < KW; ++i) L += s_ml[i][col][1] * att_weight(s_ml[i][col][0], M, A.c);
-        const float f = att_weight(st.m, M, A.c);
-        st.m = M;
-        st.l = L;
-        // wave w adds up dims [w*D/4, +D/4): every wave leaves its O in shared memory, 32 dims at a time
-        float *so = reinterpret_cast<float *>(smem);         // [4 waves][32 rows][32 dims + 1]
-        constexpr int DQ = D / 32;
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<float4 *>(o + db * 32 + 2 * e + 4 * hi) = make_float4(O[db][e], O[db][e + 1], O[db][e + 2], O[db][e + 3]);
+        } else {
+            const float inv = 1.0f / st.l;
+            uint16_t *o = A.out + (((int64_t)b * A.T + t) * A.H + h) * D;
 #pragma unroll
-        for (int db = 0; db < DQ; ++db) {
+            for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) so[(w * 32 + col) * 33 + (e & 3) + 8 * (e >> 2) + 4 * hi] = O[db][e] * f;
-            __syncthreads();
-            if (w == 0) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int at = col * 33 + (e & 3) + 8 * (e >> 2) + 4 * hi;
-                    O[db][e] = (so[at] + so[at + 32 * 33]) + (so[at + 64 * 33] + so[at + 96 * 33]);
+                for (int e = 0; e < 16; e += 4) {
+                    uint2 x = make_uint2(0, 0);
+                    if (p >= 0) x = make_uint2(att_pack<BF>(O[db][e] * inv, O[db][e + 1] * inv), att_pack<BF>(O[db][e + 2] * inv, O[db][e + 3] * inv));
+                    *reinterpret_cast<uint2 *>(o + db * 32 + 2 * e + 4 * hi) = x;
                 }
-            }
-            __syncthreads();
         }
-        if (w != 0) return;
+        return;
     }
-
-    // ---- out
-    if (r >= R) return;
-    if (A.slots) {
-        const int64_t row = ((int64_t)b * A.H + h) * A.T + t;
-        float *ml = A.part_ml + (row * A.slots + it.slot) * 2, *o = A.part_o + (row * A.slots + it.slot) * D;
-        if (hi == 0) { ml[0] = st.m; ml[1] = n + t < 0 ? -1.0f : st.l; }       // -1: the row sees nothing
+    // ---- the four waves' states over their keys, joined: rows of O in shared memory (their pitch of D + 4 words spreads the 16-byte writes over
+    // the banks), then a thread per four dims of a row
+    __shared__ float s_ml[4][32][2];
+    __syncthreads();                                         // nobody reads tiles any more
+    float *so = reinterpret_cast<float *>(smem);
+    if (r < R) {
+        if (hi == 0) { s_ml[w][col][0] = st.m; s_ml[w][col][1] = p < 0 ? -1.0f : st.l; }
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<float4 *>(o + db * 32 + 2 * e + 4 * hi) = make_float4(O[db][e], O[db][e + 1], O[db][e + 2], O[db][e + 3]);
-    } else {
-        const float inv = p < 0 ? 0.0f : 1.0f / st.l;
-        uint16_t *o = A.out + (((int64_t)b * A.T + t) * A.H + h) * D;
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                uint2 x = make_uint2(0, 0);
-                if (p >= 0) x = make_uint2(att_pack<BF>(O[db][e] * inv, O[db][e + 1] * inv), att_pack<BF>(O[db][e + 2] * inv, O[db][e + 3] * inv));
-                *reinterpret_cast<uint2 *>(o + db * 32 + 2 * e + 4 * hi) = x;
-            }
+                *reinterpret_cast<float4 *>(so + (w * 32 + col) * (D + 4) + db * 32 + 2 * e + 4 * hi) = make_float4(O[db][e], O[db][e + 1], O[db][e + 2], O[db][e + 3]);
     }
+    __syncthreads();
+    const int rows = min(32, R - it.row0);
+    for (int i = tid; i < rows * (D / 4); i += ATT_THREADS) {
+        const int k = i / (D / 4), d = i % (D / 4) * 4;
+        const float M = fmaxf(fmaxf(s_ml[0][k][0], s_ml[1][k][0]), fmaxf(s_ml[2][k][0], s_ml[3][k][0]));
+        float L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float f = att_weight(s_ml[j][k][0], M, A.c);
+            const float4 y = *reinterpret_cast<const float4 *>(so + (j * 32 + k) * (D + 4) + d);
+            L = __builtin_fmaf(s_ml[j][k][1], f, L);
+            x[0] = __builtin_fmaf(y.x, f, x[0]); x[1] = __builtin_fmaf(y.y, f, x[1]); x[2] = __builtin_fmaf(y.z, f, x[2]); x[3] = __builtin_fmaf(y.w, f, x[3]);
+        }
+        const bool none = s_ml[0][k][1] < 0.0f;
+        const int q = it.row0 + k, qb = it.packed ? q / TG : it.b, qtg = it.packed ? q - qb * TG : q, qt = qtg / A.G, qh = it.hk * A.G + qtg - qt * A.G;
+        if (A.slots) {
+            const int64_t row = ((int64_t)qb * A.H + qh) * A.T + qt;
+            float *ml = A.part_ml + (row * A.slots + it.slot) * 2, *o = A.part_o + (row * A.slots + it.slot) * D;
+            if (d == 0) { ml[0] = M; ml[1] = none ? -1.0f : L; }
+            *reinterpret_cast<float4 *>(o + d) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+            const float inv = 1.0f / L;
+            uint2 y = make_uint2(0, 0);
+            if (!none) y = make_uint2(att_pack<BF>(x[0] * inv, x[1] * inv), att_pack<BF>(x[2] * inv, x[3] * inv));
+            *reinterpret_cast<uint2 *>(A.out + (((int64_t)qb * A.T + qt) * A.H + qh) * D + d) = y;
+        }
+    }
+}
+
+// RWP: shape of the items over all requests' rows (a shared prefix), RW: of the others
+template <int D, bool BF, int RWP, int RW>
+__global__ void __launch_bounds__(ATT_THREADS, D <= 128 ? 2 : 1) attend_kernel(const AttendArgs A)
+{
+    __shared__ __attribute__((aligned(16))) uint16_t smem[256 * D + 1024];         // tiles: 256 rows of D; the joined rows: 4 * 32 * (D + 4) floats
+    const AttItem it = att_item<RWP, RW>(A);
+    if (RWP == RW) att_item_body<D, BF, RW>(A, it, smem);
+    else if (it.packed) att_item_body<D, BF, RWP>(A, it, smem);
+    else att_item_body<D, BF, RW>(A, it, smem);
 }
 
 // The slices of a row, joined: out = sum 2^(c (m_i - M)) O_i / sum 2^(c (m_i - M)) l_i.  A wave per row, D / 64 dims per lane; then the lengths
@@ -545,7 +632,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs A, in
 }
 
 // ---- how a call is cut.  Shared by the entry points and fastkv_attend_workspace_bytes.
-struct AttPlan { int rw, packed_tiles, packed_split, tiles, split, slots; int64_t blocks; };
+struct AttPlan { int rwp, rw, packed_tiles, packed_split, tiles, split, slots; int64_t blocks; };
 
 static AttPlan att_plan(int B, int H, int Hkv, int T, int64_t keys, int64_t prefix, bool advance)
 {
@@ -560,17 +647,17 @@ static AttPlan att_plan(int B, int H, int Hkv, int T, int64_t keys, int64_t pref
     };
     if (prefix > 0 && TG < 128 && B > 1) {                    // rows of all requests in one tile: the prefix is read once, not once per request
         const int64_t R = B * TG;
-        P.rw = R <= 32 ? 1 : 4;
-        const int per = 32 * P.rw;
-        P.packed_tiles = (int)((R + per - 1) / per);
-        P.packed_split = cut((int64_t)Hkv * P.packed_tiles, prefix, P.rw == 1 ? 128 : 64);
-        P.tiles = (int)((TG + per - 1) / per);
+        P.rwp = R <= 32 ? 1 : 4;
+        P.rw = TG <= 32 ? 1 : 4;
+        P.packed_tiles = (int)((R + 32 * P.rwp - 1) / (32 * P.rwp));
+        P.packed_split = cut((int64_t)Hkv * P.packed_tiles, prefix, P.rwp == 1 ? 128 : 64);
+        P.tiles = (int)((TG + 32 * P.rw - 1) / (32 * P.rw));
         P.split = 1;
         P.slots = P.packed_split + 1;
         P.blocks = (int64_t)Hkv * P.packed_tiles * P.packed_split + (int64_t)B * Hkv * P.tiles;
         return P;
     }
-    P.rw = TG <= 32 ? 1 : 4;
+    P.rwp = P.rw = TG <= 32 ? 1 : 4;
     const int per = 32 * P.rw;
     P.tiles = (int)((TG + per - 1) / per);
     P.split = cut((int64_t)B * Hkv * P.tiles, keys + prefix, P.rw == 1 ? 128 : 64);
@@ -596,8 +683,10 @@ static int att_launch(AttendArgs &A, const AttPlan &P, int advance, int32_t *len
 {
     {
         ProfScope ps_(K_ATTEND, st);
-        if (P.rw == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 1>), dim3((unsigned)P.blocks), dim3(ATT_THREADS), 0, st, A);
-        else hipLaunchKernelGGL((attend_kernel<D, BF, 4>), dim3((unsigned)P.blocks), dim3(ATT_THREADS), 0, st, A);
+        const dim3 grid((unsigned)P.blocks), block(ATT_THREADS);
+        if (P.rwp == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 1, 1>), grid, block, 0, st, A);
+        else if (P.rw == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 4, 1>), grid, block, 0, st, A);
+        else hipLaunchKernelGGL((attend_kernel<D, BF, 4, 4>), grid, block, 0, st, A);
     }
     if (hipGetLastError() != hipSuccess) return FASTKV_ELAUNCH;
     if (!A.slots) return FASTKV_OK;
@@ -622,6 +711,8 @@ static int att_run(AttendArgs &A, int dtype, int D, int64_t keys, int advance, i
     A.slot0 = P.packed_split;
     A.tiles = P.tiles;
     A.split = P.split;
+    A.near_rows = true;
+    for (int64_t r : {A.k_r, A.v_r, A.k0_r, A.v0_r}) A.near_rows = A.near_rows && r >= 0 && r < (int64_t)1 << 23;
     A.part_o = (float *)workspace;
     A.part_ml = A.part_o + (size_t)A.B * A.H * A.T * P.slots * D;
     hipStream_t st = (hipStream_t)stream;
