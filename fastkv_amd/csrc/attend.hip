@@ -23,6 +23,7 @@
 //   keys      <= 32 rows (single tokens): each wave has its own 32-key tiles and running state, merged at the end; a wave's tile is
 //             private, so the loop has no barrier and eight waves of a compute unit keep ~128 KB of loads in flight
 // Work too small to fill the chip is cut along the keys; slices leave {m, l, O} in a workspace and attend_join adds them up.
+#include <initializer_list>
 #include "fk_device.h"
 #include "fk_host.h"
 #include "prof.h"
@@ -726,10 +727,16 @@ static bool att_shape_ok(int dtype, int B, int H, int Hkv, int D, int T, int row
     return (dtype == FASTKV_F16 || dtype == FASTKV_BF16) && B >= 1 && Hkv >= 1 && H >= Hkv && H % Hkv == 0 && T >= 1 && rows >= 1 &&
            (int64_t)B * H * T <= 0x7fffffff && rows <= 0x3fffffff && D >= 1;
 }
-static bool att_rows_ok(const void *p, const int64_t *s, int n)                  // 16-byte rows
+// 16-byte rows of [n0,n1,n2] or [n1,n2]; along an extent of one nothing is stepped, whatever stride the caller has for it: it becomes 0 in `to`
+static bool att_rows_ok(const void *p, const int64_t *s, std::initializer_list<int> extents, std::initializer_list<int64_t *> to)
 {
     if (!p || !s || ((uintptr_t)p & 15)) return false;
-    for (int i = 0; i < n; ++i) if (s[i] & 7) return false;
+    auto t = to.begin();
+    for (int n : extents) {
+        if (n > 1 && (*s & 7)) return false;
+        **t++ = n > 1 ? *s : 0;
+        ++s;
+    }
     return true;
 }
 
@@ -753,15 +760,16 @@ int fastkv_window_attention(int32_t dtype, int32_t B, int32_t H, int32_t Hkv, in
 {
     if (!att_shape_ok(dtype, B, H, Hkv, D, T, rows)) return FASTKV_EINVAL;
     if (D != 64 && D != 128 && D != 256) return FASTKV_EUNSUPPORTED;
-    if (!att_rows_ok(q, q_strides, 3) || !att_rows_ok(k, k_strides, 3) || !att_rows_ok(v, v_strides, 3) || !out || ((uintptr_t)out & 15)) return FASTKV_EINVAL;
-    if (window < 0 || sinks < 0 || !(scaling > 0.0f) || scaling > 3.0e38f || len_step < 0 || len_step > 1 || (advance && !len_dev)) return FASTKV_EINVAL;
     AttendArgs A = {};
+    if (!att_rows_ok(q, q_strides, {B, H, T}, {&A.q_b, &A.q_h, &A.q_t}) || !att_rows_ok(k, k_strides, {B, Hkv, rows}, {&A.k_b, &A.k_h, &A.k_r}) ||
+        !att_rows_ok(v, v_strides, {B, Hkv, rows}, {&A.v_b, &A.v_h, &A.v_r}) || !out || ((uintptr_t)out & 15))
+        return FASTKV_EINVAL;
+    if (window < 0 || sinks < 0 || !(scaling > 0.0f) || scaling > 3.0e38f || len_step < 0 || len_step > 1 || (advance && !len_dev)) return FASTKV_EINVAL;
     A.q = (const uint16_t *)q;
-    A.q_b = q_strides[0]; A.q_h = q_strides[1]; A.q_t = q_strides[2];
     A.k = A.k0 = (const uint16_t *)k;
-    A.k_b = A.k0_b = k_strides[0]; A.k_h = A.k0_h = k_strides[1]; A.k_r = A.k0_r = k_strides[2];
+    A.k0_b = A.k_b; A.k0_h = A.k_h; A.k0_r = A.k_r;
     A.v = A.v0 = (const uint16_t *)v;
-    A.v_b = A.v0_b = v_strides[0]; A.v_h = A.v0_h = v_strides[1]; A.v_r = A.v0_r = v_strides[2];
+    A.v0_b = A.v_b; A.v0_h = A.v_h; A.v0_r = A.v_r;
     A.len = len_dev;
     A.len_step = len_step;
     A.len_all = rows - T;
@@ -781,21 +789,18 @@ int fastkv_shared_prefix_attention(int32_t dtype, int32_t B, int32_t H, int32_t 
 {
     if (!att_shape_ok(dtype, B, H, Hkv, D, T, rows) || prefix_rows < 1 || prefix_rows > 0x3fffffff) return FASTKV_EINVAL;
     if (D != 64 && D != 128 && D != 256) return FASTKV_EUNSUPPORTED;
-    if (!att_rows_ok(q, q_strides, 3) || !att_rows_ok(k, k_strides, 3) || !att_rows_ok(v, v_strides, 3) || !att_rows_ok(k_prefix, kp_strides, 2) ||
-        !att_rows_ok(v_prefix, vp_strides, 2) || !out || ((uintptr_t)out & 15))
+    AttendArgs A = {};
+    if (!att_rows_ok(q, q_strides, {B, H, T}, {&A.q_b, &A.q_h, &A.q_t}) || !att_rows_ok(k, k_strides, {B, Hkv, rows}, {&A.k_b, &A.k_h, &A.k_r}) ||
+        !att_rows_ok(v, v_strides, {B, Hkv, rows}, {&A.v_b, &A.v_h, &A.v_r}) ||
+        !att_rows_ok(k_prefix, kp_strides, {Hkv, prefix_rows}, {&A.k0_h, &A.k0_r}) ||
+        !att_rows_ok(v_prefix, vp_strides, {Hkv, prefix_rows}, {&A.v0_h, &A.v0_r}) || !out || ((uintptr_t)out & 15))
         return FASTKV_EINVAL;
     if (!(scaling > 0.0f) || scaling > 3.0e38f || !len_dev || len_step < 0 || len_step > 1) return FASTKV_EINVAL;
-    AttendArgs A = {};
     A.q = (const uint16_t *)q;
-    A.q_b = q_strides[0]; A.q_h = q_strides[1]; A.q_t = q_strides[2];
     A.k0 = (const uint16_t *)k_prefix;
-    A.k0_h = kp_strides[0]; A.k0_r = kp_strides[1];
     A.v0 = (const uint16_t *)v_prefix;
-    A.v0_h = vp_strides[0]; A.v0_r = vp_strides[1];
     A.k = (const uint16_t *)k;
-    A.k_b = k_strides[0]; A.k_h = k_strides[1]; A.k_r = k_strides[2];
     A.v = (const uint16_t *)v;
-    A.v_b = v_strides[0]; A.v_h = v_strides[1]; A.v_r = v_strides[2];
     A.len = len_dev;
     A.len_step = len_step;
     A.B = B; A.H = H; A.Hkv = Hkv; A.T = T; A.rows = rows;

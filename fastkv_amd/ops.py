@@ -458,84 +458,97 @@ def decode_gemv(x: torch.Tensor, weights, norm_weight: Optional[torch.Tensor] = 
 # ------------------------------------------------------------------------------------------------- attention forms over a cache
 _ATTEND_DTYPE = {torch.float16: 0, torch.bfloat16: 1}
 _LOGITS_DTYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_S3, _S4 = ctypes.c_int64 * 3, ctypes.c_int64 * 4
+_current_device = torch.cuda.current_device
+# (a one-token call is over in a few microseconds: the lookup of a Stream object would be a fifth of it)
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _on_device(what: str, dev: torch.device, tensors) -> None:
     # (kernels are launched on `dev`'s current stream; nothing here has a backward pass, and none is faked)
     grad = torch.is_grad_enabled()
+    cuda = dev.type == "cuda"
     for t in tensors:
-        if t is None:
-            continue
-        if t.device != dev or dev.type != "cuda":
-            raise RuntimeError(f"fastkv_amd.{what}: all tensors must be on one ROCm device (no CPU fallback exists)")
-        if grad and t.requires_grad:
-            raise RuntimeError(f"fastkv_amd.{what} has no backward pass: call it under torch.no_grad()")
+        if t is not None:
+            if not cuda or t.device != dev:
+                raise RuntimeError(f"fastkv_amd.{what}: all tensors must be on one ROCm device (no CPU fallback exists)")
+            if grad and t.requires_grad:
+                raise RuntimeError(f"fastkv_amd.{what} has no backward pass: call it under torch.no_grad()")
 
 
-def _element_strides(t: torch.Tensor):
-    # of all but the head dim; a dimension of one row is never stepped along, whatever stride torch shows for it
-    n = t.dim() - 1
-    return (ctypes.c_int64 * n)(*[t.stride(i) if t.shape[i] > 1 else 0 for i in range(n)])
+def _launch(what, dev, fn, *args) -> None:
+    """fn(*args, stream) with `dev` as the current device and its current stream."""
+    index = dev.index
+    if index == _current_device():
+        rc = fn(*args, _stream_of(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream_of(index))
+    if rc:
+        check(rc, what)
 
 
-def _device_stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-def _check_attend(what, q, k, v, len_dev, extra=()):
-    _on_device(what, q.device, (q, k, v, len_dev) + tuple(extra))
-    if q.dtype not in _ATTEND_DTYPE:
-        raise TypeError(f"fastkv_amd.{what}: fp16 or bf16 tensors expected, got {q.dtype}")
-    if any(t.dtype != q.dtype for t in (k, v) + tuple(extra)):
+def _attend(what, q, k, v, len_dev, window, sinks, scaling, advance, k_prefix=None, v_prefix=None):
+    """The checks, output, scratch and call of the three attention forms.  Output and scratch come from the caching allocator in every call:
+    nothing is kept between calls, so calls on several streams and captured graphs (whose scratch lives in their own pool) cannot meet
+    in one workspace."""
+    dev, dtype = q.device, q.dtype
+    _on_device(what, dev, (q, k, v, len_dev, k_prefix, v_prefix))
+    code = _ATTEND_DTYPE.get(dtype)
+    if code is None:
+        raise TypeError(f"fastkv_amd.{what}: fp16 or bf16 tensors expected, got {dtype}")
+    shape, kshape = q.shape, k.shape
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError(f"fastkv_amd.{what}: q, k and v must have one type")
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or k.shape[1] == 0 \
-            or q.shape[1] % k.shape[1]:
-        raise ValueError(f"fastkv_amd.{what}: expected q [B,H,T,D] and k, v [B,Hkv,rows,D], H a multiple of Hkv; got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    if q.stride(3) != 1 or k.stride(3) != 1 or v.stride(3) != 1:
+    if len(shape) != 4 or len(kshape) != 4 or kshape != v.shape or kshape[0] != shape[0] or kshape[3] != shape[3] or kshape[1] == 0 \
+            or shape[1] % kshape[1]:
+        raise ValueError(f"fastkv_amd.{what}: expected q [B,H,T,D] and k, v [B,Hkv,rows,D], H a multiple of Hkv; got {tuple(shape)}, "
+                         f"{tuple(kshape)}, {tuple(v.shape)}")
+    B, H, T, D = shape
+    _, Hkv, rows, _ = kshape
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if qs[3] != 1 or ks[3] != 1 or vs[3] != 1:
         raise ValueError(f"fastkv_amd.{what}: unit head_dim stride expected")
-    if len_dev is not None and (len_dev.dtype != torch.int32 or len_dev.dim() != 1 or len_dev.shape[0] not in (1, q.shape[0])
-                                or not len_dev.is_contiguous()):
-        raise ValueError(f"fastkv_amd.{what}: len_dev must be a contiguous int32 tensor of 1 or {q.shape[0]} lengths")
-
-
-def _run_attend(what, call, q, rows, window, sinks, prefix, Hkv, advance):
-    """Output and scratch come from the caching allocator in every call: nothing is kept between calls, so calls on several streams and
-    captured graphs (whose scratch lives in their own pool) cannot meet in one workspace."""
-    B, H, T, D = q.shape
-    out = torch.empty(B, T, H * D, dtype=q.dtype, device=q.device)
+    if rows == 0:
+        raise ValueError(f"fastkv_amd.{what}: a cache of no rows")
+    length, step = None, 0
+    if len_dev is not None:
+        if len_dev.dtype is not torch.int32 or len_dev.dim() != 1 or len_dev.shape[0] not in (1, B) or not len_dev.is_contiguous():
+            raise ValueError(f"fastkv_amd.{what}: len_dev must be a contiguous int32 tensor of 1 or {B} lengths")
+        length, step = len_dev.data_ptr(), 1 if len_dev.shape[0] > 1 else 0
+    P = 0
+    if k_prefix is not None:
+        if k_prefix.dim() == 4 and k_prefix.shape[0] == 1 and v_prefix.dim() == 4 and v_prefix.shape[0] == 1:
+            k_prefix, v_prefix = k_prefix[0], v_prefix[0]
+        if k_prefix.dtype is not dtype or v_prefix.dtype is not dtype:
+            raise TypeError(f"fastkv_amd.{what}: q, k and v must have one type")
+        if k_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape or k_prefix.shape[0] != Hkv or k_prefix.shape[2] != D or k_prefix.shape[1] == 0 \
+                or k_prefix.stride(2) != 1 or v_prefix.stride(2) != 1:
+            raise ValueError(f"fastkv_amd.{what}: expected prefixes [{Hkv},P >= 1,{D}] with unit head_dim stride, got {tuple(k_prefix.shape)}, "
+                             f"{tuple(v_prefix.shape)}")
+        P = k_prefix.shape[1]
+    out = torch.empty((B, T, H * D), dtype=dtype, device=dev)
     if out.numel() == 0:
         return out
-    need = load().fastkv_attend_workspace_bytes(B, H, Hkv, D, T, rows, window, sinks, prefix, 1 if advance else 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    ptr = ws.data_ptr() if need else None
-    if q.device.index == torch.cuda.current_device():
-        check(call(out.data_ptr(), ptr, need, _device_stream(q.device)), what)
+    lib = load()
+    adv = 1 if advance else 0
+    need = lib.fastkv_attend_workspace_bytes(B, H, Hkv, D, T, rows, window, sinks, P, adv)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    wp = ws.data_ptr() if need else None
+    if P:
+        _launch(what, dev, lib.fastkv_shared_prefix_attention, code, B, H, Hkv, D, T, q.data_ptr(), _S4(*qs), k_prefix.data_ptr(),
+                _S3(*k_prefix.stride()), v_prefix.data_ptr(), _S3(*v_prefix.stride()), P, k.data_ptr(), _S4(*ks), v.data_ptr(), _S4(*vs), rows,
+                length, step, adv, scaling, out.data_ptr(), wp, need)
     else:
-        with torch.cuda.device(q.device):
-            check(call(out.data_ptr(), ptr, need, _device_stream(q.device)), what)
+        _launch(what, dev, lib.fastkv_window_attention, code, B, H, Hkv, D, T, q.data_ptr(), _S4(*qs), k.data_ptr(), _S4(*ks), v.data_ptr(),
+                _S4(*vs), rows, length, step, adv, window, sinks, scaling, out.data_ptr(), wp, need)
     return out
 
 
-def _window_attention(what, q, k, v, window, sinks, scaling, len_dev, advance):
-    _check_attend(what, q, k, v, len_dev)
-    B, H, T, D = q.shape
-    Hkv, rows = k.shape[1], k.shape[2]
+def _window_of(what, window, sinks):
     if window is not None and window < 1 or sinks < 0:
         raise ValueError(f"fastkv_amd.{what}: window >= 1 (None: no window) and sinks >= 0 expected, got {window}, {sinks}")
-    if rows == 0:
-        raise ValueError(f"fastkv_amd.{what}: a cache of no rows")
-    window, sinks = min(window or 0, 2 ** 30), min(sinks, 2 ** 30)
-    scaling = D ** -0.5 if scaling is None else scaling
-
-    def call(out, ws, nbytes, stream):
-        return load().fastkv_window_attention(_ATTEND_DTYPE[q.dtype], B, H, Hkv, D, T, q.data_ptr(), _element_strides(q), k.data_ptr(),
-                                              _element_strides(k), v.data_ptr(), _element_strides(v), rows,
-                                              len_dev.data_ptr() if len_dev is not None else None,
-                                              1 if len_dev is not None and len_dev.shape[0] > 1 else 0, 1 if advance else 0, window, sinks,
-                                              scaling, out, ws, nbytes, stream)
-
-    return _run_attend(what, call, q, rows, window, sinks, 0, Hkv, advance)
+    return min(window or 0, 1 << 30), min(sinks, 1 << 30)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
@@ -544,7 +557,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     bf16 (any strides, unit head_dim stride) -> [B,T,H*D].  Query t of request b stands at p = len_dev[b] + t and sees the rows j <= p
     with j < sinks or j > p - window; `window` None: all j <= p.  `len_dev` (int32 [B] or [1], on the device): rows in front of the T
     new ones, whose K / V are already in rows len .. len+T-1; None: the last T of all rows.  p < 0 (left padding): zeros."""
-    return _window_attention("window_attention", q, k, v, window, sinks, scaling, len_dev, False)
+    window, sinks = _window_of("window_attention", window, sinks)
+    return _attend("window_attention", q, k, v, len_dev, window, sinks, q.shape[-1] ** -0.5 if scaling is None else scaling, False)
 
 
 def decode_window_attention(q: torch.Tensor, kslab: torch.Tensor, vslab: torch.Tensor, len_dev: torch.Tensor, scaling: float,
@@ -552,11 +566,13 @@ def decode_window_attention(q: torch.Tensor, kslab: torch.Tensor, vslab: torch.T
     """`decode_attention` for a model with a sliding window: q [B,H,1,D] over the slab rows that `window` and `sinks` leave of rows
     0 .. len_dev (inclusive: the row decode_append just wrote) -> [B,1,H*D]; len_dev (int32 [1] or [B]) moves on by one on the device
     unless `advance` is False.  A negative length is an idle request: zeros, and it stays.  Only the visible rows are read."""
+    what = "decode_window_attention"
     if q.dim() != 4 or q.shape[2] != 1:
-        raise ValueError(f"fastkv_amd.decode_window_attention: one token per request expected, got q {tuple(q.shape)}")
+        raise ValueError(f"fastkv_amd.{what}: one token per request expected, got q {tuple(q.shape)}")
     if len_dev is None:
-        raise ValueError("fastkv_amd.decode_window_attention: len_dev expected")
-    return _window_attention("decode_window_attention", q, kslab, vslab, window, sinks, scaling, len_dev, advance)
+        raise ValueError(f"fastkv_amd.{what}: len_dev expected")
+    window, sinks = _window_of(what, window, sinks)
+    return _attend(what, q, kslab, vslab, len_dev, window, sinks, scaling, advance)
 
 
 def decode_shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, kslab: torch.Tensor, vslab: torch.Tensor,
@@ -566,29 +582,28 @@ def decode_shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_pr
     request's own rows j <= len_dev[b] + t (the T new rows are already written there); the prefix is read once for the batch.
     len_dev (int32 [1] or [B]) moves on by T on the device unless `advance` is False; len_dev[b] + t < 0 is idle: zeros."""
     what = "decode_shared_prefix_attention"
-    if k_prefix.dim() == 4 and k_prefix.shape[0] == 1 and v_prefix.dim() == 4 and v_prefix.shape[0] == 1:
-        k_prefix, v_prefix = k_prefix[0], v_prefix[0]
-    _check_attend(what, q, kslab, vslab, len_dev, (k_prefix, v_prefix))
-    if len_dev is None:
-        raise ValueError(f"fastkv_amd.{what}: len_dev expected")
-    B, H, T, D = q.shape
-    Hkv, rows = kslab.shape[1], kslab.shape[2]
-    if k_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape or k_prefix.shape[0] != Hkv or k_prefix.shape[2] != D or k_prefix.shape[1] == 0 \
-            or k_prefix.stride(2) != 1 or v_prefix.stride(2) != 1:
-        raise ValueError(f"fastkv_amd.{what}: expected prefixes [{Hkv},P >= 1,{D}] with unit head_dim stride, got {tuple(k_prefix.shape)}, "
-                         f"{tuple(v_prefix.shape)}")
-    if T > rows:
-        raise ValueError(f"fastkv_amd.{what}: {T} new tokens in slabs of {rows} rows")
-    P = k_prefix.shape[1]
+    if len_dev is None or k_prefix is None or v_prefix is None:
+        raise ValueError(f"fastkv_amd.{what}: a prefix and len_dev expected")
+    if q.dim() == 4 and kslab.dim() == 4 and q.shape[2] > kslab.shape[2]:
+        raise ValueError(f"fastkv_amd.{what}: {q.shape[2]} new tokens in slabs of {kslab.shape[2]} rows")
+    return _attend(what, q, kslab, vslab, len_dev, 0, 0, scaling, advance, k_prefix, v_prefix)
 
-    def call(out, ws, nbytes, stream):
-        return load().fastkv_shared_prefix_attention(_ATTEND_DTYPE[q.dtype], B, H, Hkv, D, T, q.data_ptr(), _element_strides(q),
-                                                     k_prefix.data_ptr(), _element_strides(k_prefix), v_prefix.data_ptr(),
-                                                     _element_strides(v_prefix), P, kslab.data_ptr(), _element_strides(kslab),
-                                                     vslab.data_ptr(), _element_strides(vslab), rows, len_dev.data_ptr(),
-                                                     1 if len_dev.shape[0] > 1 else 0, 1 if advance else 0, scaling, out, ws, nbytes, stream)
 
-    return _run_attend(what, call, q, rows, 0, 0, P, Hkv, advance)
+def _per_row(t, dtype, B, what, name):
+    if t is None:
+        return None, 0
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] not in (1, B) or not t.is_contiguous():
+        raise ValueError(f"fastkv_amd.{what}: {name} must be a contiguous {dtype} tensor of 1 or {B} values")
+    return t.data_ptr(), 1 if t.shape[0] > 1 else 0
+
+
+def _row_table(t, dtype, B, width, what, name):
+    if t is None:
+        return None, 0
+    if t.dtype is not dtype or t.dim() not in (1, 2) or t.shape[-1] != width or (t.dim() == 2 and t.shape[0] not in (1, B)) \
+            or (width > 1 and t.stride(-1) != 1):
+        raise ValueError(f"fastkv_amd.{what}: {name} must be {dtype} [{width}], [1,{width}] or [{B},{width}] with unit stride")
+    return t.data_ptr(), t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else 0
 
 
 def decode_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, n_tokens: Optional[torch.Tensor] = None,
@@ -604,53 +619,33 @@ def decode_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None
     frequency fp32 [B] or [1]; bias fp32 [V], [1,V] or [B,V]; allowed int32 [words], [1,words] or [B,words], words = ceil(V/32); all on the
     device.  `out`: where the result goes (`logits` itself: in place); a new tensor if None."""
     what = "decode_penalties"
-    if logits.dim() != 2 or logits.dtype not in _LOGITS_DTYPE or logits.shape[1] == 0 or logits.stride(1) != 1:
+    code = _LOGITS_DTYPE.get(logits.dtype)
+    if code is None or logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"fastkv_amd.{what}: logits [B,V >= 1] in fp16, bf16 or fp32 with unit stride expected, got {tuple(logits.shape)} {logits.dtype}")
     B, V = logits.shape
     dev = logits.device
     _on_device(what, dev, (logits, tokens, n_tokens, n_prompt, repetition, presence, frequency, bias, allowed, out))
-
-    def per_row(t, dtype, name):
-        if t is None:
-            return None, 0
-        if t.dtype != dtype or t.dim() != 1 or t.shape[0] not in (1, B) or not t.is_contiguous():
-            raise ValueError(f"fastkv_amd.{what}: {name} must be a contiguous {dtype} tensor of 1 or {B} values")
-        return t.data_ptr(), 1 if t.shape[0] > 1 else 0
-
-    def rows_of(t, dtype, width, name):
-        if t is None:
-            return None, 0
-        if t.dtype != dtype or t.dim() not in (1, 2) or t.shape[-1] != width or (t.dim() == 2 and t.shape[0] not in (1, B)) or t.stride(-1) != 1:
-            raise ValueError(f"fastkv_amd.{what}: {name} must be {dtype} [{width}], [1,{width}] or [{B},{width}] with unit stride")
-        return t.data_ptr(), t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else 0
-
+    L, tp, ts = 0, None, 0
     if tokens is None:
         if not (repetition is presence is frequency is n_tokens is n_prompt is None):
             raise ValueError(f"fastkv_amd.{what}: penalties need the history in `tokens`")
-    elif tokens.dtype != torch.int64 or tokens.dim() != 2 or tokens.shape[0] != B or (tokens.shape[1] > 1 and tokens.stride(1) != 1):
-        raise ValueError(f"fastkv_amd.{what}: tokens must be int64 [{B},L] with unit stride")
+    else:
+        if tokens.dtype is not torch.int64 or tokens.dim() != 2 or tokens.shape[0] != B or (tokens.shape[1] > 1 and tokens.stride(1) != 1):
+            raise ValueError(f"fastkv_amd.{what}: tokens must be int64 [{B},L] with unit stride")
+        L = tokens.shape[1]
+        if L:
+            tp, ts = tokens.data_ptr(), tokens.stride(0) if B > 1 else 0
     if out is None:
-        out = torch.empty(B, V, dtype=logits.dtype, device=dev)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.stride(1) != 1:
+        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
+    elif out.shape != logits.shape or out.dtype is not logits.dtype or (V > 1 and out.stride(1) != 1):
         raise ValueError(f"fastkv_amd.{what}: out must be a {logits.dtype} tensor [{B},{V}] with unit stride")
     if B == 0:
         return out
-    args = per_row(n_tokens, torch.int32, "n_tokens") + per_row(n_prompt, torch.int32, "n_prompt") + \
-        per_row(repetition, torch.float32, "repetition") + per_row(presence, torch.float32, "presence") + \
-        per_row(frequency, torch.float32, "frequency") + rows_of(bias, torch.float32, V, "bias") + \
-        rows_of(allowed, torch.int32, (V + 31) // 32, "allowed")
-    L = tokens.shape[1] if tokens is not None else 0
-
-    def call():
-        return load().fastkv_decode_penalties(_LOGITS_DTYPE[logits.dtype], B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V,
-                                              tokens.data_ptr() if L else None, tokens.stride(0) if L else 0, L, *args, out.data_ptr(),
-                                              out.stride(0) if B > 1 else V, _device_stream(dev))
-
-    if dev.index == torch.cuda.current_device():
-        check(call(), what)
-    else:
-        with torch.cuda.device(dev):
-            check(call(), what)
+    _launch(what, dev, load().fastkv_decode_penalties, code, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, tp, ts, L,
+            *_per_row(n_tokens, torch.int32, B, what, "n_tokens"), *_per_row(n_prompt, torch.int32, B, what, "n_prompt"),
+            *_per_row(repetition, torch.float32, B, what, "repetition"), *_per_row(presence, torch.float32, B, what, "presence"),
+            *_per_row(frequency, torch.float32, B, what, "frequency"), *_row_table(bias, torch.float32, B, V, what, "bias"),
+            *_row_table(allowed, torch.int32, B, (V + 31) // 32, what, "allowed"), out.data_ptr(), out.stride(0) if B > 1 else V)
     return out
 
 
