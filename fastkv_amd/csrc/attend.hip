@@ -85,6 +85,10 @@ template <bool BF> __device__ __forceinline__ bool att_wild(uint32_t w)
     const uint32_t e = BF ? 0x7f80u : 0x7c00u;
     return (w & e) == e || (w >> 16 & e) == e;
 }
+template <bool BF> __device__ __forceinline__ bool att_wild_piece(att_u4 x)
+{
+    return att_wild<BF>(x[0]) || att_wild<BF>(x[1]) || att_wild<BF>(x[2]) || att_wild<BF>(x[3]);
+}
 // x of both halves' lanes of a column (the pair's words are copied out first: a bit cast of a vector element reads element 0 here)
 struct AttPair { uint32_t lo, hi; };
 __device__ __forceinline__ AttPair att_halves(float x)
@@ -182,14 +186,18 @@ template <int D, int NB, int NW> struct AttLoad {
             }
         }
     }
-    // this lane's V pieces, landed: which rows hold an infinity or NaN
-    template <bool BF> static __device__ __forceinline__ void scan(const uint16_t *vs, int w, unsigned long long *wild)
+    // This lane's V pieces, landed, of a tile that some row does not see all of: an infinity or NaN must not touch the rows that do not see it
+    // (0 * inf), so a piece that holds one is taken out of the tile, its row is noted, and att_wild_rows adds it for the rows that see it.
+    template <bool BF> static __device__ __forceinline__ void scan(uint16_t *vs, int w, unsigned long long *wild)
     {
         const int lane = threadIdx.x & 63;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < CH; ++i) {
-            const att_u4 x = *reinterpret_cast<const att_u4 *>(vs + (i * NW + w) * RPI * D + lane * 8);
-            if (att_wild<BF>(x[0]) || att_wild<BF>(x[1]) || att_wild<BF>(x[2]) || att_wild<BF>(x[3])) atomicOr(wild, 1ull << row_of(i, w, lane));
+            att_u4 *at = reinterpret_cast<att_u4 *>(vs + (i * NW + w) * RPI * D + lane * 8);
+            if (att_wild_piece<BF>(*at)) {
+                *at = att_u4{0, 0, 0, 0};
+                atomicOr(wild, 1ull << row_of(i, w, lane));
+            }
         }
     }
 };
@@ -242,7 +250,7 @@ __device__ __forceinline__ void att_softmax(att_f16 (&S)[NB], att_u4 (&P)[NB * 2
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) tm = fmaxf(tm, S[kb][r]);
+        for (int r = 0; r < 16; ++r) tm = __builtin_elementwise_maximum(tm, S[kb][r]);
     tm = att_other_half_max(tm);
     if (__any((tm - st.m) * c > ATT_GROWTH)) {
         const float mn = fmaxf(st.m, tm);
@@ -268,14 +276,11 @@ __device__ __forceinline__ void att_softmax(att_f16 (&S)[NB], att_u4 (&P)[NB * 2
     st.l += l0 + l1;
 }
 
-// O^T += V^T P^T.  `wild`: keys of the tile (bits) whose V row holds an infinity or NaN, given where some row does not see some key -- a row
-// must not be touched by a key that it does not see (0 * inf), so these keys are taken out of the product and added for the rows that see them.
-template <int D, bool BF, int NB>
-__device__ __forceinline__ void att_values(const uint16_t *vs, const att_u4 (&P)[NB * 2], att_f16 (&O)[D / 32], const AttKeys &K, int u0, int p,
-                                           uint64_t wild)
+// O^T += V^T P^T
+template <int D, bool BF, int NB> __device__ __forceinline__ void att_values(const uint16_t *vs, const att_u4 (&P)[NB * 2], att_f16 (&O)[D / 32])
 {
     // lane i of a group of 16 addresses row i / 4, elements 4 * (i % 4) of a 4 x 16 block and receives column i
-    const int lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5, gi = lane & 15, krow = gi >> 2;
+    const int lane = threadIdx.x & 63, hi = lane >> 5, gi = lane & 15, krow = gi >> 2;
     const int piece = (lane >> 4 & 1) * 2 + (gi >> 1 & 1), sw = att_swz(4 * hi + krow);
     typedef __attribute__((address_space(3))) att_s4 lds_s4;
     const uint16_t *at[2];                   // dims 32 db + 8 piece + ..: the swizzle is in the low three bits of 4 db + piece
@@ -289,17 +294,19 @@ __device__ __forceinline__ void att_values(const uint16_t *vs, const att_u4 (&P)
             const att_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)v);
             const att_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(v + 8 * D));
             const uint2 xa = __builtin_bit_cast(uint2, x), ya = __builtin_bit_cast(uint2, y);
-            att_u4 a = {xa.x, xa.y, ya.x, ya.y};
-            if (wild) {
-                const uint32_t cut = (uint32_t)(wild >> (s * 16 + 4 * hi)), b = (cut & 0xfu) | (cut >> 4 & 0xf0u);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] &= (b >> (2 * e) & 1 ? 0u : 0xffffu) | (b >> (2 * e + 1) & 1 ? 0u : 0xffff0000u);
-            }
-            O[db] = att_mfma<BF>(a, P[s], O[db]);
+            O[db] = att_mfma<BF>(att_u4{xa.x, xa.y, ya.x, ya.y}, P[s], O[db]);
         }
     }
-    for (uint64_t left = wild; left; left &= left - 1) {
-        const int key = __builtin_ctzll(left);
+}
+
+// the pieces that AttLoad::scan took out of a tile, for the rows that see their keys (bits of `wild`)
+template <int D, bool BF, int NB>
+__device__ __forceinline__ void att_wild_rows(const att_u4 (&P)[NB * 2], att_f16 (&O)[D / 32], const AttKeys &K, int u0, int p, uint64_t wild)
+{
+    const int lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
+#pragma unroll 1
+    for (; wild; wild &= wild - 1) {
+        const int key = __builtin_ctzll(wild), u = u0 + key;
         uint32_t w = 0;
 #pragma unroll
         for (int s = 0; s < NB * 2; ++s)
@@ -309,13 +316,18 @@ __device__ __forceinline__ void att_values(const uint16_t *vs, const att_u4 (&P)
         w = (uint32_t)__shfl((int)w, col + 32 * (key >> 2 & 1), 64);
         const float pk = att_float<BF>(key & 1 ? w >> 16 : w & 0xffffu);
         const bool seen = AttSees(K, u0, p)(key);
+        const uint16_t *row = u < K.n0 ? K.v0 + u * K.v0_r : K.v + (int64_t)(K.lo + u - K.n0) * K.v_r;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int d = db * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi;
-                const float x = att_float<BF>(vs[key * D + ((d >> 3) ^ att_swz(key)) * 8 + (d & 7)]);
-                O[db][r] = seen ? __builtin_fmaf(pk, x, O[db][r]) : O[db][r];
+            for (int e = 0; e < 16; e += 4) {    // dims 32 db + 2 e + 4 hi .. + 3: half of a piece
+                const att_u4 x = *reinterpret_cast<const att_u4 *>(row + db * 32 + 2 * e);
+                const bool add = seen & att_wild_piece<BF>(x);
+                const uint32_t a = hi ? x[2] : x[0], b = hi ? x[3] : x[1];
+                const float v[4] = {att_float<BF>(a & 0xffffu), att_float<BF>(a >> 16), att_float<BF>(b & 0xffffu), att_float<BF>(b >> 16)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) O[db][e + i] = add ? __builtin_fmaf(pk, v[i], O[db][e + i]) : O[db][e + i];
+                asm volatile("" ::: "memory");   // (one piece at a time: this is rare, its registers are not)
             }
     }
 }
@@ -466,7 +478,8 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
                 const bool mx = mixed(u, p_lo, p_hi);
                 att_scores<D, BF, NB>(cur, Q, S);
                 att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, mx || u + KT > K.N);
-                att_values<D, BF, NB>(cur + TILE, P, O, K, u, p, mx ? s_wild[i % 3] : 0);
+                att_values<D, BF, NB>(cur + TILE, P, O);
+                if (mixed(u, e_lo, e_hi)) att_wild_rows<D, BF, NB>(P, O, K, u, p, s_wild[i % 3]);
             }
             att_landed<0>();
             if (i + 1 < nt && mixed(u + KT, e_lo, e_hi)) Load::template scan<BF>(nxt + TILE, w, &s_wild[(i + 1) % 3]);
@@ -501,7 +514,8 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
                 asm volatile("" ::: "memory");
                 wild = s_wild[w];
             }
-            att_values<D, BF, NB>(vs, P, O, K, u, p, wild);
+            att_values<D, BF, NB>(vs, P, O);
+            if (mx) att_wild_rows<D, BF, NB>(P, O, K, u, p, wild);
             att_read_done();
             if (more) Load::issue(K, un, true, vs, 0);
         }

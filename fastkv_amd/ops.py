@@ -464,25 +464,23 @@ _current_device = torch.cuda.current_device
 _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _on_device(what: str, dev: torch.device, tensors) -> None:
-    # (kernels are launched on `dev`'s current stream; nothing here has a backward pass, and none is faked)
+def _on_device(what: str, index: int, tensors) -> None:
+    # (kernels are launched on that device's current stream; nothing here has a backward pass, and none is faked)
     grad = torch.is_grad_enabled()
-    cuda = dev.type == "cuda"
     for t in tensors:
         if t is not None:
-            if not cuda or t.device != dev:
+            if t.get_device() != index or index < 0:
                 raise RuntimeError(f"fastkv_amd.{what}: all tensors must be on one ROCm device (no CPU fallback exists)")
             if grad and t.requires_grad:
                 raise RuntimeError(f"fastkv_amd.{what} has no backward pass: call it under torch.no_grad()")
 
 
-def _launch(what, dev, fn, *args) -> None:
-    """fn(*args, stream) with `dev` as the current device and its current stream."""
-    index = dev.index
+def _launch(what, index, fn, *args) -> None:
+    """fn(*args, stream) with device `index` as the current one, on its current stream."""
     if index == _current_device():
         rc = fn(*args, _stream_of(index))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             rc = fn(*args, _stream_of(index))
     if rc:
         check(rc, what)
@@ -492,8 +490,8 @@ def _attend(what, q, k, v, len_dev, window, sinks, scaling, advance, k_prefix=No
     """The checks, output, scratch and call of the three attention forms.  Output and scratch come from the caching allocator in every call:
     nothing is kept between calls, so calls on several streams and captured graphs (whose scratch lives in their own pool) cannot meet
     in one workspace."""
-    dev, dtype = q.device, q.dtype
-    _on_device(what, dev, (q, k, v, len_dev, k_prefix, v_prefix))
+    index, dtype = q.get_device(), q.dtype
+    _on_device(what, index, (q, k, v, len_dev, k_prefix, v_prefix))
     code = _ATTEND_DTYPE.get(dtype)
     if code is None:
         raise TypeError(f"fastkv_amd.{what}: fp16 or bf16 tensors expected, got {dtype}")
@@ -527,6 +525,7 @@ def _attend(what, q, k, v, len_dev, window, sinks, scaling, advance, k_prefix=No
             raise ValueError(f"fastkv_amd.{what}: expected prefixes [{Hkv},P >= 1,{D}] with unit head_dim stride, got {tuple(k_prefix.shape)}, "
                              f"{tuple(v_prefix.shape)}")
         P = k_prefix.shape[1]
+    dev = q.device
     out = torch.empty((B, T, H * D), dtype=dtype, device=dev)
     if out.numel() == 0:
         return out
@@ -536,11 +535,11 @@ def _attend(what, q, k, v, len_dev, window, sinks, scaling, advance, k_prefix=No
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     wp = ws.data_ptr() if need else None
     if P:
-        _launch(what, dev, lib.fastkv_shared_prefix_attention, code, B, H, Hkv, D, T, q.data_ptr(), _S4(*qs), k_prefix.data_ptr(),
+        _launch(what, index, lib.fastkv_shared_prefix_attention, code, B, H, Hkv, D, T, q.data_ptr(), _S4(*qs), k_prefix.data_ptr(),
                 _S3(*k_prefix.stride()), v_prefix.data_ptr(), _S3(*v_prefix.stride()), P, k.data_ptr(), _S4(*ks), v.data_ptr(), _S4(*vs), rows,
                 length, step, adv, scaling, out.data_ptr(), wp, need)
     else:
-        _launch(what, dev, lib.fastkv_window_attention, code, B, H, Hkv, D, T, q.data_ptr(), _S4(*qs), k.data_ptr(), _S4(*ks), v.data_ptr(),
+        _launch(what, index, lib.fastkv_window_attention, code, B, H, Hkv, D, T, q.data_ptr(), _S4(*qs), k.data_ptr(), _S4(*ks), v.data_ptr(),
                 _S4(*vs), rows, length, step, adv, window, sinks, scaling, out.data_ptr(), wp, need)
     return out
 
@@ -623,8 +622,8 @@ def decode_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None
     if code is None or logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"fastkv_amd.{what}: logits [B,V >= 1] in fp16, bf16 or fp32 with unit stride expected, got {tuple(logits.shape)} {logits.dtype}")
     B, V = logits.shape
-    dev = logits.device
-    _on_device(what, dev, (logits, tokens, n_tokens, n_prompt, repetition, presence, frequency, bias, allowed, out))
+    index = logits.get_device()
+    _on_device(what, index, (logits, tokens, n_tokens, n_prompt, repetition, presence, frequency, bias, allowed, out))
     L, tp, ts = 0, None, 0
     if tokens is None:
         if not (repetition is presence is frequency is n_tokens is n_prompt is None):
@@ -636,12 +635,12 @@ def decode_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None
         if L:
             tp, ts = tokens.data_ptr(), tokens.stride(0) if B > 1 else 0
     if out is None:
-        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
+        out = torch.empty((B, V), dtype=logits.dtype, device=logits.device)
     elif out.shape != logits.shape or out.dtype is not logits.dtype or (V > 1 and out.stride(1) != 1):
         raise ValueError(f"fastkv_amd.{what}: out must be a {logits.dtype} tensor [{B},{V}] with unit stride")
     if B == 0:
         return out
-    _launch(what, dev, load().fastkv_decode_penalties, code, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, tp, ts, L,
+    _launch(what, index, load().fastkv_decode_penalties, code, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, tp, ts, L,
             *_per_row(n_tokens, torch.int32, B, what, "n_tokens"), *_per_row(n_prompt, torch.int32, B, what, "n_prompt"),
             *_per_row(repetition, torch.float32, B, what, "repetition"), *_per_row(presence, torch.float32, B, what, "presence"),
             *_per_row(frequency, torch.float32, B, what, "frequency"), *_row_table(bias, torch.float32, B, V, what, "bias"),
