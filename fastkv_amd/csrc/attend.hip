@@ -23,7 +23,9 @@
 //   keys      <= 32 rows (single tokens): each wave has its own 32-key tiles and running state, merged at the end; a wave's tile is
 //             private, so the loop has no barrier and eight waves of a compute unit keep ~128 KB of loads in flight
 // Work too small to fill the chip is cut along the keys; slices leave {m, l, O} in a workspace and attend_join adds them up.
+#include <limits.h>
 #include <initializer_list>
+#include <type_traits>
 #include "fk_device.h"
 #include "fk_host.h"
 #include "prof.h"
@@ -123,7 +125,17 @@ struct AttKeys {                             // the keys of one item, and which 
     int64_t k0_r, v0_r, k_r, v_r;
     int n0, lo, N;                           // segment 0; first row of segment 1; all
     int window, sinks;
-    bool near_rows;                          // 64 rows of any of the four lie within 31 bits of bytes
+    int lean0, lean1, lean2;                 // tiles in [.., lean0) or [lean1, lean2): see lean()
+
+    // Tiles of KT keys that lie in one segment, whole, and are seen by all rows at positions a .. z; `near_rows`: 64 rows of any of the four
+    // lie within 31 bits of bytes.  Nearly all tiles are such; what is not is looked at key by key.
+    __device__ __forceinline__ void find_lean(int KT, bool near_rows, int a, int z)
+    {
+        lean0 = near_rows ? min(n0, N) - KT + 1 : INT_MIN;
+        lean1 = max(n0, z - window + 1 - lo + n0);
+        lean2 = near_rows ? min(N, a + 1 - lo + n0) - KT + 1 : INT_MIN;
+    }
+    __device__ __forceinline__ bool lean(int u) const { return u < lean0 || (u >= lean1 && u < lean2); }
 };
 
 // Which keys a row at position p >= 0 sees, by their number from u0 on: k < end, and k < first (segment 0 and sinks) or k > before (the window).
@@ -142,49 +154,75 @@ struct AttSees {
 
 struct AttState { float m, l; };
 
+// 16 bytes per active lane from memory to shared memory: lane l's land at lds + OFF + 16 l.  Written as assembly because the compiler, which
+// cannot tell the tile in flight from the one being read, waits for every such load in front of the next transposing read; the waits are
+// att_landed's, and nothing of these loads is in a register.
+template <int OFF> __device__ __forceinline__ void att_bring(att_u4 buffer, int offset, int base_offset, uint32_t lds)
+{
+    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(lds), "v"(offset), "s"(buffer), "s"(base_offset), "n"(OFF) : "memory", "scc");
+}
+template <int OFF> __device__ __forceinline__ void att_bring(const uint16_t *src, uint32_t lds)
+{
+    asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(src), "n"(OFF) : "memory", "scc");
+}
+template <int I, int N, class F> __device__ __forceinline__ void att_each(F &&f)      // f(0) .. f(N - 1), the index a constant
+{
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>());
+        att_each<I + 1, N>(f);
+    }
+}
+__device__ __forceinline__ uint32_t att_uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+
 // Rows u0 .. u0 + 32*NB - 1 of K and V on their way to shared memory, brought by NW waves without passing registers (the 16 bytes of lane l
 // land at a wave's base + 16 l; the swizzle is in which piece of the row the lane asks for).
 template <int D, int NB, int NW> struct AttLoad {
     static constexpr int KT = 32 * NB, C = D / 8, RPI = 64 / C, CH = KT / (RPI * NW);     // rows per instruction, instructions per wave
     static constexpr int NV = RPI * NW >= 8 ? 1 : 8 / (RPI * NW);                         // distinct swizzles over a lane's rows
-    typedef __attribute__((address_space(3))) uint32_t lds_u32;
-    typedef __attribute__((address_space(1))) uint32_t glb_u32;
+    static constexpr int STEP = NW * RPI * D * 2;                                         // bytes from one instruction's rows to the next's
 
     static __device__ __forceinline__ int row_of(int i, int w, int lane) { return (i * NW + w) * RPI + lane / C; }
-    static __device__ __forceinline__ bool plain(const AttKeys &K, int u0) { return K.near_rows && u0 + KT <= K.N && (u0 + KT <= K.n0 || u0 >= K.n0); }
-
-    // Whole tiles of one segment: buffer loads, a 32-bit offset per lane and the tile's base in scalar registers.  Others (the tile over
-    // the segments' seam, the last one, rows further apart than 32 bits reach): an address per lane, and zeros behind the last key -- their
-    // scores are cut off, but a V row there must be finite.
-    static __device__ __forceinline__ void issue(const AttKeys &K, int u0, bool value, uint16_t *dst, int w)
+    static __device__ __forceinline__ uint32_t lds_of(const uint16_t *dst, int w)
+    {
+        return att_uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)dst + w * RPI * D * 2);
+    }
+    // A whole tile of rows row, row + 1, ... of `base`: a 32-bit offset per lane, the tile's base in scalar registers
+    static __device__ __forceinline__ void plain(const uint16_t *base, int64_t r, int row, uint32_t lds, int w)
+    {
+        const int lane = threadIdx.x & 63, step = (int)r * 2;
+        const uintptr_t at = (uintptr_t)(base + (row + w * RPI) * r);
+        const att_u4 buffer = {att_uniform((uint32_t)at), att_uniform((uint32_t)(at >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
+        att_each<0, CH>([&](auto I) {
+            constexpr int i = I;
+            const int c = (lane % C) ^ att_swz(row_of(i % NV, w, lane));
+            att_bring<i * STEP>(buffer, lane / C * step + c * 16, (int)att_uniform(i * NW * RPI * step), lds);
+        });
+    }
+    // Any other tile (over the segments' seam, the last one, rows further apart than 32 bits reach): an address per lane, and zeros behind the
+    // last key -- their scores are cut off, but a V row there must be finite.
+    static __device__ __forceinline__ void any(const AttKeys &K, int u0, bool value, uint16_t *dst, int w)
     {
         const int lane = threadIdx.x & 63;
-        const bool first = u0 + KT <= K.n0;
-        if (plain(K, u0)) {
-            const int64_t r = value ? (first ? K.v0_r : K.v_r) : (first ? K.k0_r : K.k_r);
-            const uint16_t *base = (value ? (first ? K.v0 : K.v) : (first ? K.k0 : K.k)) + (first ? u0 : K.lo + u0 - K.n0) * r;
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(base), 0, 0x7fffffff, 0x00020000);
-            const int step = (int)r * 2;
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int c = (lane % C) ^ att_swz(row_of(i % NV, w, lane));
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_u32 *)(dst + (i * NW + w) * RPI * D), 16, lane / C * step + c * 16,
-                                                         (i * NW + w) * RPI * step, 0, 0);
+        const uint32_t lds = lds_of(dst, w);
+        att_each<0, CH>([&](auto I) {
+            constexpr int i = I;
+            const int row = row_of(i, w, lane), u = u0 + row, c = (lane % C) ^ att_swz(row);
+            if (u < K.N) {
+                const bool f = u < K.n0;
+                const int64_t j = f ? u : K.lo + u - K.n0;
+                att_bring<i * STEP>((value ? (f ? K.v0 : K.v) + j * (f ? K.v0_r : K.v_r) : (f ? K.k0 : K.k) + j * (f ? K.k0_r : K.k_r)) + c * 8, lds);
+            } else {
+                *reinterpret_cast<att_u4 *>(dst + (i * NW + w) * RPI * D + lane * 8) = att_u4{0, 0, 0, 0};
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int row = row_of(i, w, lane), u = u0 + row, c = (lane % C) ^ att_swz(row);
-                if (u < K.N) {
-                    const bool f = u < K.n0;
-                    const int64_t j = f ? u : K.lo + u - K.n0;
-                    const uint16_t *src = (value ? (f ? K.v0 : K.v) + j * (f ? K.v0_r : K.v_r) : (f ? K.k0 : K.k) + j * (f ? K.k0_r : K.k_r)) + c * 8;
-                    __builtin_amdgcn_global_load_lds((const glb_u32 *)src, (lds_u32 *)(dst + (i * NW + w) * RPI * D), 16, 0, 0);
-                } else {
-                    *reinterpret_cast<att_u4 *>(dst + (i * NW + w) * RPI * D + lane * 8) = att_u4{0, 0, 0, 0};
-                }
-            }
-        }
+        });
+    }
+    // the tile at u0: `lean` as AttKeys::lean says
+    static __device__ __forceinline__ void issue(const AttKeys &K, int u0, bool lean, bool value, uint16_t *dst, int w)
+    {
+        if (!lean) any(K, u0, value, dst, w);
+        else if (u0 < K.n0) plain(value ? K.v0 : K.k0, value ? K.v0_r : K.k0_r, u0, lds_of(dst, w), w);
+        else plain(value ? K.v : K.k, value ? K.v_r : K.k_r, K.lo + u0 - K.n0, lds_of(dst, w), w);
     }
     // This lane's V pieces, landed, of a tile that some row does not see all of: an infinity or NaN must not touch the rows that do not see it
     // (0 * inf), so a piece that holds one is taken out of the tile, its row is noted, and att_wild_rows adds it for the rows that see it.
@@ -401,7 +439,6 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
     // ---- the item's keys
     AttKeys K;
     int p_lo = 0, p_hi = 0, e_lo = 0, e_hi = 0;              // positions of this wave's rows, of the workgroup's
-    K.near_rows = A.near_rows;
     K.k0_r = A.k0_r;
     K.v0_r = A.v0_r;
     K.k_r = A.k_r;
@@ -436,12 +473,7 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
         u_lo = min(K.N, it.slice * per * KT * KW);
         K.N = min(K.N, u_lo + per * KT * KW);
     }
-    // rows at positions a .. z: some of them does not see some key in the tile at u (keys behind the last one aside)
-    auto mixed = [&](int u, int a, int z) {
-        if (u + KT <= K.n0) return false;
-        const int j = K.lo + max(u, K.n0) - K.n0, j1 = K.lo + min(u + KT, K.N) - K.n0;
-        return j1 - 1 > a || j <= z - K.window;
-    };
+    K.find_lean(KT, A.near_rows, e_lo, e_hi);
     AttState st = {-INFINITY, 0.0f};
     att_f16 O[D / 32], S[NB];
     att_u4 P[NB * 2];
@@ -452,62 +484,72 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
 
     if (RW == 4) {
         typedef AttLoad<D, NB, 4> Load;
-        if (tid < 3) s_wild[tid] = 0;
-        const int nt = (K.N - u_lo + KT - 1) / KT;
-        if (nt > 0) {
-            Load::issue(K, u_lo, false, smem, w);
-            Load::issue(K, u_lo, true, smem + TILE, w);
+        const bool idle = wrow0 >= R;
+        bool lean = u_lo < K.N && K.lean(u_lo);
+        if (tid == 0) s_wild[0] = 0;
+        if (u_lo < K.N) {
+            Load::issue(K, u_lo, lean, false, smem, w);
+            Load::issue(K, u_lo, lean, true, smem + TILE, w);
         }
         att_landed<0>();
         __syncthreads();
-        if (nt > 0 && mixed(u_lo, e_lo, e_hi)) Load::template scan<BF>(smem + TILE, w, &s_wild[0]);
-        __syncthreads();
-        for (int i = 0; i < nt; ++i) {
-            const int u = u_lo + i * KT;
-            uint16_t *cur = smem + (i & 1) * 2 * TILE, *nxt = smem + (i & 1 ^ 1) * 2 * TILE;
-            if (i + 1 < nt) {                                 // (the other buffer was last read before the barrier)
-                Load::issue(K, u + KT, false, nxt, w);
-                Load::issue(K, u + KT, true, nxt + TILE, w);
+        if (!lean) {
+            if (u_lo < K.N) Load::template scan<BF>(smem + TILE, w, &s_wild[0]);
+            __syncthreads();
+        }
+        int at = 0;                                           // the tile's place in shared memory
+        for (int u = u_lo; u < K.N; u += KT) {
+            const uint16_t *cur = smem + at;
+            uint16_t *nxt = smem + (at ^ 2 * TILE);
+            const int un = u + KT;
+            const bool more = un < K.N, next_lean = K.lean(un);
+            if (more) {                                       // (the other buffer was last read before the barrier)
+                if (!next_lean && tid == 0) s_wild[at ? 0 : 1] = 0;
+                Load::issue(K, un, next_lean, false, nxt, w);
+                Load::issue(K, un, next_lean, true, nxt + TILE, w);
             }
-            bool skip = wrow0 >= R;                           // no rows, or a tile that none of them sees
-            if (!it.packed && u >= K.n0) {
+            bool skip = idle;
+            if (!lean && !it.packed && u >= K.n0) {           // a tile that none of this wave's rows sees
                 const int j = K.lo + u - K.n0;
                 skip = skip || j > p_hi || (j + KT - 1 <= p_lo - K.window && j >= K.sinks);
             }
             if (!skip) {
-                const bool mx = mixed(u, p_lo, p_hi);
                 att_scores<D, BF, NB>(cur, Q, S);
-                att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, mx || u + KT > K.N);
+                att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, !lean);
                 att_values<D, BF, NB>(cur + TILE, P, O);
-                if (mixed(u, e_lo, e_hi)) att_wild_rows<D, BF, NB>(P, O, K, u, p, s_wild[i % 3]);
+                if (!lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, s_wild[at ? 1 : 0]);
             }
             att_landed<0>();
-            if (i + 1 < nt && mixed(u + KT, e_lo, e_hi)) Load::template scan<BF>(nxt + TILE, w, &s_wild[(i + 1) % 3]);
-            if (tid == 0) s_wild[(i + 2) % 3] = 0;           // last read a tile ago, written a tile from now
             __syncthreads();
+            if (more && !next_lean) {
+                Load::template scan<BF>(nxt + TILE, w, &s_wild[at ? 0 : 1]);
+                __syncthreads();
+            }
+            at ^= 2 * TILE;
+            lean = next_lean;
         }
     } else {
         typedef AttLoad<D, NB, 1> Load;
         uint16_t *ks = smem + w * 2 * TILE, *vs = ks + TILE;
         int u = u_lo + w * KT;
+        bool lean = K.lean(u);
         if (u < K.N) {
-            Load::issue(K, u, false, ks, 0);
-            Load::issue(K, u, true, vs, 0);
+            Load::issue(K, u, lean, false, ks, 0);
+            Load::issue(K, u, lean, true, vs, 0);
         }
-        for (; u < K.N; u += KT * KW) {
+        while (u < K.N) {
             const int un = u + KT * KW;
-            const bool more = un < K.N;
-            if (Load::plain(K, u)) att_landed<Load::CH>();
+            const bool more = un < K.N, next_lean = more && K.lean(un);
+            if (lean) att_landed<Load::CH>();                // (a lean tile's V is exactly CH loads behind its K)
             else att_landed<0>();
             att_scores<D, BF, NB>(ks, Q, S);
             att_read_done();
-            if (more) Load::issue(K, un, false, ks, 0);
-            const bool mx = mixed(u, p_lo, p_hi);
-            att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, mx || u + KT > K.N);
-            if (more && Load::plain(K, un)) att_landed<Load::CH>();
+            if (more) Load::issue(K, un, next_lean, false, ks, 0);
+            att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, !lean);
+            if (next_lean) att_landed<Load::CH>();
             else att_landed<0>();
             uint64_t wild = 0;
-            if (mx) {
+            if (!lean && p_lo != p_hi) {                     // (rows at one position see the same keys)
                 if (lane == 0) s_wild[w] = 0;
                 asm volatile("" ::: "memory");
                 Load::template scan<BF>(vs, 0, &s_wild[w]);  // (one wave's accesses to shared memory are in order)
@@ -515,9 +557,11 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
                 wild = s_wild[w];
             }
             att_values<D, BF, NB>(vs, P, O);
-            if (mx) att_wild_rows<D, BF, NB>(P, O, K, u, p, wild);
+            if (!lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, wild);
             att_read_done();
-            if (more) Load::issue(K, un, true, vs, 0);
+            if (more) Load::issue(K, un, next_lean, true, vs, 0);
+            u = un;
+            lean = next_lean;
         }
     }
     st.l = att_other_half_sum(st.l);
