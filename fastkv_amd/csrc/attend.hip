@@ -112,9 +112,13 @@ __device__ __forceinline__ float att_other_half_sum(float x)
     const AttPair p = att_halves(x);
     return __builtin_bit_cast(float, p.lo) + __builtin_bit_cast(float, p.hi);
 }
-// 16-byte piece c of row `row` lies at piece c ^ att_swz(row): eight consecutive rows' equal pieces (the K reads), and the piece pairs of
-// four consecutive rows (the transposing V reads), fall on different banks
-__device__ __forceinline__ int att_swz(int row) { return (row & 3) << 1 | (row >> 2 & 1); }
+// 16-byte piece c of row `row` of a tile lies at piece c ^ att_swz: shared memory serves 16 pieces (64 banks) at a time.  K: equal pieces of 16
+// consecutive rows fall on different banks; V: four pieces in a row of each of four consecutive rows do (and eight rows on, all is the same).
+template <int D, bool V> __device__ __forceinline__ int att_swz(int row)
+{
+    if (D == 64) return V ? (row >> 1 & 1) << 2 | (row >> 2 & 1) : (row >> 1 & 1) << 2 | (row >> 2 & 3);       // two rows are one turn of the banks
+    return V ? (row & 3) << 2 | (row >> 2 & 1) : (row & 3) << 2 | (row >> 2 & 3);
+}
 
 // what a partial sum over keys of maximum m counts for beside the maximum M of all of them (no key at all: both are -inf; a NaN among
 // the sums survives a weight of zero, as it survives in the formula)
@@ -179,7 +183,7 @@ __device__ __forceinline__ uint32_t att_uniform(uint32_t x) { return (uint32_t)_
 // land at a wave's base + 16 l; the swizzle is in which piece of the row the lane asks for).
 template <int D, int NB, int NW> struct AttLoad {
     static constexpr int KT = 32 * NB, C = D / 8, RPI = 64 / C, CH = KT / (RPI * NW);     // rows per instruction, instructions per wave
-    static constexpr int NV = RPI * NW >= 8 ? 1 : 8 / (RPI * NW);                         // distinct swizzles over a lane's rows
+    static constexpr int NV = RPI * NW >= 16 ? 1 : 16 / (RPI * NW);                       // distinct swizzles over a lane's rows
     static constexpr int STEP = NW * RPI * D * 2;                                         // bytes from one instruction's rows to the next's
 
     static __device__ __forceinline__ int row_of(int i, int w, int lane) { return (i * NW + w) * RPI + lane / C; }
@@ -188,41 +192,41 @@ template <int D, int NB, int NW> struct AttLoad {
         return att_uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)dst + w * RPI * D * 2);
     }
     // A whole tile of rows row, row + 1, ... of `base`: a 32-bit offset per lane, the tile's base in scalar registers
-    static __device__ __forceinline__ void plain(const uint16_t *base, int64_t r, int row, uint32_t lds, int w)
+    template <bool V> static __device__ __forceinline__ void plain(const uint16_t *base, int64_t r, int row, uint32_t lds, int w)
     {
         const int lane = threadIdx.x & 63, step = (int)r * 2;
         const uintptr_t at = (uintptr_t)(base + (row + w * RPI) * r);
         const att_u4 buffer = {att_uniform((uint32_t)at), att_uniform((uint32_t)(at >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
         att_each<0, CH>([&](auto I) {
             constexpr int i = I;
-            const int c = (lane % C) ^ att_swz(row_of(i % NV, w, lane));
+            const int c = (lane % C) ^ att_swz<D, V>(row_of(i % NV, w, lane));
             att_bring<i * STEP>(buffer, lane / C * step + c * 16, (int)att_uniform(i * NW * RPI * step), lds);
         });
     }
     // Any other tile (over the segments' seam, the last one, rows further apart than 32 bits reach): an address per lane, and zeros behind the
     // last key -- their scores are cut off, but a V row there must be finite.
-    static __device__ __forceinline__ void any(const AttKeys &K, int u0, bool value, uint16_t *dst, int w)
+    template <bool V> static __device__ __forceinline__ void any(const AttKeys &K, int u0, uint16_t *dst, int w)
     {
         const int lane = threadIdx.x & 63;
         const uint32_t lds = lds_of(dst, w);
         att_each<0, CH>([&](auto I) {
             constexpr int i = I;
-            const int row = row_of(i, w, lane), u = u0 + row, c = (lane % C) ^ att_swz(row);
+            const int row = row_of(i, w, lane), u = u0 + row, c = (lane % C) ^ att_swz<D, V>(row);
             if (u < K.N) {
                 const bool f = u < K.n0;
                 const int64_t j = f ? u : K.lo + u - K.n0;
-                att_bring<i * STEP>((value ? (f ? K.v0 : K.v) + j * (f ? K.v0_r : K.v_r) : (f ? K.k0 : K.k) + j * (f ? K.k0_r : K.k_r)) + c * 8, lds);
+                att_bring<i * STEP>((V ? (f ? K.v0 : K.v) + j * (f ? K.v0_r : K.v_r) : (f ? K.k0 : K.k) + j * (f ? K.k0_r : K.k_r)) + c * 8, lds);
             } else {
                 *reinterpret_cast<att_u4 *>(dst + (i * NW + w) * RPI * D + lane * 8) = att_u4{0, 0, 0, 0};
             }
         });
     }
     // the tile at u0: `lean` as AttKeys::lean says
-    static __device__ __forceinline__ void issue(const AttKeys &K, int u0, bool lean, bool value, uint16_t *dst, int w)
+    template <bool V> static __device__ __forceinline__ void issue(const AttKeys &K, int u0, bool lean, uint16_t *dst, int w)
     {
-        if (!lean) any(K, u0, value, dst, w);
-        else if (u0 < K.n0) plain(value ? K.v0 : K.k0, value ? K.v0_r : K.k0_r, u0, lds_of(dst, w), w);
-        else plain(value ? K.v : K.k, value ? K.v_r : K.k_r, K.lo + u0 - K.n0, lds_of(dst, w), w);
+        if (!lean) any<V>(K, u0, dst, w);
+        else if (u0 < K.n0) plain<V>(V ? K.v0 : K.k0, V ? K.v0_r : K.k0_r, u0, lds_of(dst, w), w);
+        else plain<V>(V ? K.v : K.k, V ? K.v_r : K.k_r, K.lo + u0 - K.n0, lds_of(dst, w), w);
     }
     // This lane's V pieces, landed, of a tile that some row does not see all of: an infinity or NaN must not touch the rows that do not see it
     // (0 * inf), so a piece that holds one is taken out of the tile, its row is noted, and att_wild_rows adds it for the rows that see it.
@@ -257,10 +261,11 @@ __device__ __forceinline__ void att_read_done()
 // S^T = K Q^T of a tile of 32*NB keys
 template <int D, bool BF, int NB> __device__ __forceinline__ void att_scores(const uint16_t *ks, const att_u4 (&Q)[D / 16], att_f16 (&S)[NB])
 {
-    const int lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5, sw = att_swz(col);
-    const uint16_t *at[4];                   // piece (2 s + hi) ^ sw of row col: the swizzle is in the low three bits
+    const int lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5, sw = att_swz<D, false>(col);
+    constexpr int NX = D == 64 ? 4 : 8;      // piece (2 s + hi) ^ sw of row col: the swizzle is in the low three or four bits
+    const uint16_t *at[NX];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) at[x] = ks + col * D + ((2 * x + hi) ^ sw) * 8;
+    for (int x = 0; x < NX; ++x) at[x] = ks + col * D + ((2 * x + hi) ^ sw) * 8;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
@@ -268,7 +273,7 @@ template <int D, bool BF, int NB> __device__ __forceinline__ void att_scores(con
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
 #pragma unroll
-        for (int kb = 0; kb < NB; ++kb) S[kb] = att_mfma<BF>(*reinterpret_cast<const att_u4 *>(at[s & 3] + (s >> 2) * 64 + kb * 32 * D), Q[s], S[kb]);
+        for (int kb = 0; kb < NB; ++kb) S[kb] = att_mfma<BF>(*reinterpret_cast<const att_u4 *>(at[s % NX] + s / NX * NX * 16 + kb * 32 * D), Q[s], S[kb]);
 }
 
 // the running softmax over a tile's scores, u0 its first key; `edge`: some row may not see some key.  P^T comes out as the second operand of V^T P^T.
@@ -319,16 +324,17 @@ template <int D, bool BF, int NB> __device__ __forceinline__ void att_values(con
 {
     // lane i of a group of 16 addresses row i / 4, elements 4 * (i % 4) of a 4 x 16 block and receives column i
     const int lane = threadIdx.x & 63, hi = lane >> 5, gi = lane & 15, krow = gi >> 2;
-    const int piece = (lane >> 4 & 1) * 2 + (gi >> 1 & 1), sw = att_swz(4 * hi + krow);
+    const int piece = (lane >> 4 & 1) * 2 + (gi >> 1 & 1), sw = att_swz<D, true>(4 * hi + krow);
     typedef __attribute__((address_space(3))) att_s4 lds_s4;
-    const uint16_t *at[2];                   // dims 32 db + 8 piece + ..: the swizzle is in the low three bits of 4 db + piece
+    constexpr int NX = D == 64 ? 2 : 4;      // dims 32 db + 8 piece + ..: the swizzle is in the low three or four bits of 4 db + piece
+    const uint16_t *at[NX];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) at[x] = vs + (4 * hi + krow) * D + ((4 * x + piece) ^ sw) * 8 + (gi & 1) * 4;
+    for (int x = 0; x < NX; ++x) at[x] = vs + (4 * hi + krow) * D + ((4 * x + piece) ^ sw) * 8 + (gi & 1) * 4;
 #pragma unroll
     for (int s = 0; s < NB * 2; ++s) {
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) {
-            const uint16_t *v = at[db & 1] + (db >> 1) * 64 + s * 16 * D;
+            const uint16_t *v = at[db % NX] + db / NX * NX * 32 + s * 16 * D;
             const att_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)v);
             const att_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(v + 8 * D));
             const uint2 xa = __builtin_bit_cast(uint2, x), ya = __builtin_bit_cast(uint2, y);
@@ -488,8 +494,8 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
         bool lean = u_lo < K.N && K.lean(u_lo);
         if (tid == 0) s_wild[0] = 0;
         if (u_lo < K.N) {
-            Load::issue(K, u_lo, lean, false, smem, w);
-            Load::issue(K, u_lo, lean, true, smem + TILE, w);
+            Load::template issue<false>(K, u_lo, lean, smem, w);
+            Load::template issue<true>(K, u_lo, lean, smem + TILE, w);
         }
         att_landed<0>();
         __syncthreads();
@@ -505,8 +511,8 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
             const bool more = un < K.N, next_lean = K.lean(un);
             if (more) {                                       // (the other buffer was last read before the barrier)
                 if (!next_lean && tid == 0) s_wild[at ? 0 : 1] = 0;
-                Load::issue(K, un, next_lean, false, nxt, w);
-                Load::issue(K, un, next_lean, true, nxt + TILE, w);
+                Load::template issue<false>(K, un, next_lean, nxt, w);
+                Load::template issue<true>(K, un, next_lean, nxt + TILE, w);
             }
             bool skip = idle;
             if (!lean && !it.packed && u >= K.n0) {           // a tile that none of this wave's rows sees
@@ -534,8 +540,8 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
         int u = u_lo + w * KT;
         bool lean = K.lean(u);
         if (u < K.N) {
-            Load::issue(K, u, lean, false, ks, 0);
-            Load::issue(K, u, lean, true, vs, 0);
+            Load::template issue<false>(K, u, lean, ks, 0);
+            Load::template issue<true>(K, u, lean, vs, 0);
         }
         while (u < K.N) {
             const int un = u + KT * KW;
@@ -544,7 +550,7 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
             else att_landed<0>();
             att_scores<D, BF, NB>(ks, Q, S);
             att_read_done();
-            if (more) Load::issue(K, un, next_lean, false, ks, 0);
+            if (more) Load::template issue<false>(K, un, next_lean, ks, 0);
             att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, !lean);
             if (next_lean) att_landed<Load::CH>();
             else att_landed<0>();
@@ -559,7 +565,7 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
             att_values<D, BF, NB>(vs, P, O);
             if (!lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, wild);
             att_read_done();
-            if (more) Load::issue(K, un, next_lean, true, vs, 0);
+            if (more) Load::template issue<true>(K, un, next_lean, vs, 0);
             u = un;
             lean = next_lean;
         }
