@@ -129,17 +129,19 @@ struct AttKeys {                             // the keys of one item, and which 
     int64_t k0_r, v0_r, k_r, v_r;
     int n0, lo, N;                           // segment 0; first row of segment 1; all
     int window, sinks;
-    int lean0, lean1, lean2;                 // tiles in [.., lean0) or [lean1, lean2): see lean()
+    int end0, end1, seen1, seen2;            // see whole(), lean()
 
-    // Tiles of KT keys that lie in one segment, whole, and are seen by all rows at positions a .. z; `near_rows`: 64 rows of any of the four
-    // lie within 31 bits of bytes.  Nearly all tiles are such; what is not is looked at key by key.
-    __device__ __forceinline__ void find_lean(int KT, bool near_rows, int a, int z)
+    // For tiles of KT keys; a .. z: the positions of all rows; near_rows: 64 rows of any of the four lie within 31 bits of bytes
+    __device__ __forceinline__ void look(int KT, bool near_rows, int a, int z)
     {
-        lean0 = near_rows ? min(n0, N) - KT + 1 : INT_MIN;
-        lean1 = max(n0, z - window + 1 - lo + n0);
-        lean2 = near_rows ? min(N, a + 1 - lo + n0) - KT + 1 : INT_MIN;
+        end0 = near_rows ? min(n0, N) - KT : INT_MIN;
+        end1 = near_rows ? N - KT : INT_MIN;
+        seen1 = max(n0, z - window + 1 - lo + n0);
+        seen2 = min(N, a + 1 - lo + n0) - KT;
     }
-    __device__ __forceinline__ bool lean(int u) const { return u < lean0 || (u >= lean1 && u < lean2); }
+    // the tile at u lies in one segment with all its keys; ... and every row sees all of them: nearly all tiles are such
+    __device__ __forceinline__ bool whole(int u) const { return u <= end0 || (u >= n0 && u <= end1); }
+    __device__ __forceinline__ bool lean(int u) const { return u <= end0 || (u >= seen1 && u <= min(seen2, end1)); }
 };
 
 // Which keys a row at position p >= 0 sees, by their number from u0 on: k < end, and k < first (segment 0 and sinks) or k > before (the window).
@@ -219,12 +221,12 @@ template <int D, int NB, int NW> struct AttLoad {
             } else {
                 *reinterpret_cast<att_u4 *>(dst + (i * NW + w) * RPI * D + lane * 8) = att_u4{0, 0, 0, 0};
             }
+            __builtin_amdgcn_sched_barrier(0);   // (one address at a time)
         });
     }
-    // the tile at u0: `lean` as AttKeys::lean says
-    template <bool V> static __device__ __forceinline__ void issue(const AttKeys &K, int u0, bool lean, uint16_t *dst, int w)
+    template <bool V> static __device__ __forceinline__ void issue(const AttKeys &K, int u0, uint16_t *dst, int w)
     {
-        if (!lean) any<V>(K, u0, dst, w);
+        if (!K.whole(u0)) any<V>(K, u0, dst, w);
         else if (u0 < K.n0) plain<V>(V ? K.v0 : K.k0, V ? K.v0_r : K.k0_r, u0, lds_of(dst, w), w);
         else plain<V>(V ? K.v : K.k, V ? K.v_r : K.k_r, K.lo + u0 - K.n0, lds_of(dst, w), w);
     }
@@ -371,7 +373,7 @@ __device__ __forceinline__ void att_wild_rows(const att_u4 (&P)[NB * 2], att_f16
                 const float v[4] = {att_float<BF>(a & 0xffffu), att_float<BF>(a >> 16), att_float<BF>(b & 0xffffu), att_float<BF>(b >> 16)};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) O[db][e + i] = add ? __builtin_fmaf(pk, v[i], O[db][e + i]) : O[db][e + i];
-                asm volatile("" ::: "memory");   // (one piece at a time: this is rare, its registers are not)
+                __builtin_amdgcn_sched_barrier(0);   // (one piece at a time: this is rare, its registers are not)
             }
     }
 }
@@ -426,7 +428,7 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
 {
     constexpr int NB = RW == 4 ? 2 : 1, KT = 32 * NB, KW = 4 / RW;
     constexpr int TILE = KT * D;                             // elements of a K (or V) tile
-    __shared__ unsigned long long s_wild[4];
+    __shared__ unsigned long long s_wild[4];                // (rows: three in turn)
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hi = lane >> 5;
     const int TG = A.T * A.G, R = it.packed ? A.B * TG : TG;
     // ---- this lane's query row
@@ -479,7 +481,7 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
         u_lo = min(K.N, it.slice * per * KT * KW);
         K.N = min(K.N, u_lo + per * KT * KW);
     }
-    K.find_lean(KT, A.near_rows, e_lo, e_hi);
+    K.look(KT, A.near_rows, e_lo, e_hi);
     AttState st = {-INFINITY, 0.0f};
     att_f16 O[D / 32], S[NB];
     att_u4 P[NB * 2];
@@ -491,28 +493,25 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
     if (RW == 4) {
         typedef AttLoad<D, NB, 4> Load;
         const bool idle = wrow0 >= R;
-        bool lean = u_lo < K.N && K.lean(u_lo);
-        if (tid == 0) s_wild[0] = 0;
+        if (tid < 3) s_wild[tid] = 0;
         if (u_lo < K.N) {
-            Load::template issue<false>(K, u_lo, lean, smem, w);
-            Load::template issue<true>(K, u_lo, lean, smem + TILE, w);
+            Load::template issue<false>(K, u_lo, smem, w);
+            Load::template issue<true>(K, u_lo, smem + TILE, w);
         }
-        att_landed<0>();
         __syncthreads();
-        if (!lean) {
-            if (u_lo < K.N) Load::template scan<BF>(smem + TILE, w, &s_wild[0]);
-            __syncthreads();
-        }
-        int at = 0;                                           // the tile's place in shared memory
+        att_landed<0>();
+        bool lean = K.lean(u_lo);
+        if (u_lo < K.N && !lean) Load::template scan<BF>(smem + TILE, w, &s_wild[0]);
+        __syncthreads();
+        int at = 0, wl = 0;                                   // the tile's place in shared memory, its word of s_wild
         for (int u = u_lo; u < K.N; u += KT) {
             const uint16_t *cur = smem + at;
             uint16_t *nxt = smem + (at ^ 2 * TILE);
-            const int un = u + KT;
+            const int un = u + KT, wn = wl == 2 ? 0 : wl + 1;
             const bool more = un < K.N, next_lean = K.lean(un);
             if (more) {                                       // (the other buffer was last read before the barrier)
-                if (!next_lean && tid == 0) s_wild[at ? 0 : 1] = 0;
-                Load::template issue<false>(K, un, next_lean, nxt, w);
-                Load::template issue<true>(K, un, next_lean, nxt + TILE, w);
+                Load::template issue<false>(K, un, nxt, w);
+                Load::template issue<true>(K, un, nxt + TILE, w);
             }
             bool skip = idle;
             if (!lean && !it.packed && u >= K.n0) {           // a tile that none of this wave's rows sees
@@ -523,36 +522,35 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
                 att_scores<D, BF, NB>(cur, Q, S);
                 att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, !lean);
                 att_values<D, BF, NB>(cur + TILE, P, O);
-                if (!lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, s_wild[at ? 1 : 0]);
+                if (!lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, s_wild[wl]);
             }
             att_landed<0>();
+            if (more && !next_lean) Load::template scan<BF>(nxt + TILE, w, &s_wild[wn]);     // (a lane looks at what it brought itself)
+            if (tid == 0) s_wild[wn == 2 ? 0 : wn + 1] = 0;  // last read a tile ago, written a tile from now
             __syncthreads();
-            if (more && !next_lean) {
-                Load::template scan<BF>(nxt + TILE, w, &s_wild[at ? 0 : 1]);
-                __syncthreads();
-            }
             at ^= 2 * TILE;
+            wl = wn;
             lean = next_lean;
         }
     } else {
         typedef AttLoad<D, NB, 1> Load;
         uint16_t *ks = smem + w * 2 * TILE, *vs = ks + TILE;
         int u = u_lo + w * KT;
-        bool lean = K.lean(u);
+        bool whole = K.whole(u);
         if (u < K.N) {
-            Load::template issue<false>(K, u, lean, ks, 0);
-            Load::template issue<true>(K, u, lean, vs, 0);
+            Load::template issue<false>(K, u, ks, 0);
+            Load::template issue<true>(K, u, vs, 0);
         }
         while (u < K.N) {
             const int un = u + KT * KW;
-            const bool more = un < K.N, next_lean = more && K.lean(un);
-            if (lean) att_landed<Load::CH>();                // (a lean tile's V is exactly CH loads behind its K)
+            const bool more = un < K.N, next_whole = more && K.whole(un), lean = K.lean(u);
+            if (whole) att_landed<Load::CH>();               // (a whole tile's V is exactly CH loads behind its K)
             else att_landed<0>();
             att_scores<D, BF, NB>(ks, Q, S);
             att_read_done();
-            if (more) Load::template issue<false>(K, un, next_lean, ks, 0);
+            if (more) Load::template issue<false>(K, un, ks, 0);
             att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, !lean);
-            if (next_lean) att_landed<Load::CH>();
+            if (next_whole) att_landed<Load::CH>();
             else att_landed<0>();
             uint64_t wild = 0;
             if (!lean && p_lo != p_hi) {                     // (rows at one position see the same keys)
@@ -565,9 +563,9 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
             att_values<D, BF, NB>(vs, P, O);
             if (!lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, wild);
             att_read_done();
-            if (more) Load::template issue<true>(K, un, next_lean, vs, 0);
+            if (more) Load::template issue<true>(K, un, vs, 0);
             u = un;
-            lean = next_lean;
+            whole = next_whole;
         }
     }
     st.l = att_other_half_sum(st.l);
@@ -650,44 +648,61 @@ __global__ void __launch_bounds__(ATT_THREADS, D <= 128 ? 2 : 1) attend_kernel(c
     else att_item_body<D, BF, RW>(A, it, smem);
 }
 
-// The slices of a row, joined: out = sum 2^(c (m_i - M)) O_i / sum 2^(c (m_i - M)) l_i.  A wave per row, D / 64 dims per lane; then the lengths
-// move on (the last reader of the old ones is behind this launch's start).
-template <int D, bool BF>
+// The slices of a row, joined: out = sum 2^(c (m_i - M)) O_i / sum 2^(c (m_i - M)) l_i.  A thread has four dims of a row; SG threads share the
+// slices of a row (8 where there are many: a few loads in flight each, instead of dozens one behind the other) and are added up in their
+// order.  Then the lengths move on: the last reader of the old ones was the launch before.
+template <int D, bool BF, int SG>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs A, int64_t nrows, int advance, int32_t *len, uint32_t *host_flag)
 {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);          // (b * H + h) * T + t
-    if (row < nrows) {
-        const float *ml = A.part_ml + row * A.slots * 2, *po = A.part_o + row * A.slots * D + lane * E;
-        float M = -INFINITY;
-        bool none = false;
-        for (int i = lane; i < A.slots; i += 64) {
-            M = fmaxf(M, ml[2 * i]);
-            none = none || ml[2 * i + 1] < 0.0f;
-        }
-        M = wave_max(M);
-        none = __any(none);
-        float L = 0.0f, o[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = 0.0f;
+    constexpr int LPR = D / 4, ROWS = 256 / (LPR * SG) > 0 ? 256 / (LPR * SG) : 1;
+    __shared__ float s_o[SG > 1 ? SG : 1][ROWS][SG > 1 ? D + 4 : 1], s_l[SG > 1 ? SG : 1][ROWS];
+    const int tid = threadIdx.x, d = tid % LPR * 4, k = tid / LPR % ROWS, sg = tid / (LPR * ROWS);
+    const int64_t row = (int64_t)blockIdx.x * ROWS + k;                        // (b * H + h) * T + t
+    const bool mine = row < nrows && sg < SG;
+    float M = -INFINITY, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    bool none = false;
+    if (mine) {
+        const float2 *ml = reinterpret_cast<const float2 *>(A.part_ml) + row * A.slots;
+        const float *po = A.part_o + row * A.slots * D + d;
+#pragma unroll 8
         for (int i = 0; i < A.slots; ++i) {
-            const float m = ml[2 * i], f = att_weight(m, M, A.c);
-            L += f * ml[2 * i + 1];
+            const float2 v = ml[i];
+            M = fmaxf(M, v.x);
+            none = none | (v.y < 0.0f);
+        }
+#pragma unroll 4
+        for (int i = sg; i < A.slots; i += SG) {
+            const float2 v = ml[i];
+            const float4 y = *reinterpret_cast<const float4 *>(po + (int64_t)i * D);
+            const float f = att_weight(v.x, M, A.c);
+            L = __builtin_fmaf(v.y, f, L);
+            x[0] = __builtin_fmaf(y.x, f, x[0]); x[1] = __builtin_fmaf(y.y, f, x[1]); x[2] = __builtin_fmaf(y.z, f, x[2]); x[3] = __builtin_fmaf(y.w, f, x[3]);
+        }
+    }
+    if (SG > 1) {
+        if (sg < SG) {
+            *reinterpret_cast<float4 *>(&s_o[sg][k][d]) = make_float4(x[0], x[1], x[2], x[3]);
+            if (d == 0) s_l[sg][k] = L;
+        }
+        __syncthreads();
+        if (sg == 0) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float x = po[(int64_t)i * D + e];
-                o[e] = __builtin_fmaf(f, x, o[e]);
+            for (int j = 1; j < SG; ++j) {
+                const float4 y = *reinterpret_cast<const float4 *>(&s_o[j][k][d]);
+                L += s_l[j][k];
+                x[0] += y.x; x[1] += y.y; x[2] += y.z; x[3] += y.w;
             }
         }
+    }
+    if (mine && sg == 0) {
         const int64_t bh = row / A.T, t = row - bh * A.T, b = bh / A.H, h = bh - b * A.H;
-        uint16_t *out = A.out + ((b * A.T + t) * A.H + h) * D + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) out[e] = none ? 0 : (uint16_t)(att_pack<BF>(o[e] / L, 0.0f) & 0xffffu);
+        uint2 y = make_uint2(0, 0);
+        if (!none) y = make_uint2(att_pack<BF>(x[0] / L, x[1] / L), att_pack<BF>(x[2] / L, x[3] / L));
+        *reinterpret_cast<uint2 *>(A.out + ((b * A.T + t) * A.H + h) * D + d) = y;
     }
     if (advance && blockIdx.x == 0) {
         const int nlen = A.len_step ? A.B : 1;
-        for (int i = threadIdx.x; i < nlen; i += 256) {
+        for (int i = tid; i < nlen; i += 256) {
             const int n = len[i];
             if (n < 0) continue;                                                // an idle request stays where it is
             len[i] = n <= A.rows - advance ? n + advance : A.rows;
@@ -699,23 +714,37 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs A, in
 // ---- how a call is cut.  Shared by the entry points and fastkv_attend_workspace_bytes.
 struct AttPlan { int rwp, rw, packed_tiles, packed_split, tiles, split, slots; int64_t blocks; };
 
-static AttPlan att_plan(int B, int H, int Hkv, int T, int64_t keys, int64_t prefix, bool advance)
+// Into how many slices the keys of `items` items (n keys each, `per` keys a step of the workgroup) are cut: the least of a plain sum of times in
+// us, whose constants are measured -- what a workgroup takes for itself (2.5) and per step (rows: 1.55 for 128 x 64 at 128 dims alone on its
+// compute unit, 2.0 each for two; keys: 1.0, and what the memory gives), and the join (3.5, and the slices' fp32 sums written and read).
+static int att_cut(int64_t items, int64_t n, int per, double step, double step2, int64_t rows, int D, int extra)
+{
+    const int64_t steps = (n + per - 1) / per;
+    const int most = (int)(steps < 64 ? steps : 64);
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= most; ++s) {
+        const int64_t wgs = items * s, each = (steps + s - 1) / s;
+        const int64_t full = wgs / 512, rest = wgs % 512;
+        double t = (double)(full * (2.5 + each * step2)) + (rest ? 2.5 + each * (rest > 256 ? step2 : step) : 0.0);
+        if (s + extra > 1) t += 3.5 + rows * (s + extra) * (D + 2) * 8.0 / 4e6;
+        if (t < least * 0.99) { least = t; best = s; }
+    }
+    return best;
+}
+
+static AttPlan att_plan(int B, int H, int Hkv, int D, int T, int64_t keys, int64_t prefix, bool advance)
 {
     AttPlan P = {};
-    const int64_t TG = (int64_t)T * (H / Hkv);
-    const int64_t want = 512;                                 // workgroups: two per compute unit
-    auto cut = [&](int64_t items, int64_t n, int64_t least) { // slices of n keys: enough to fill the chip, none shorter than `least`
-        int64_t s = (want + items - 1) / items;
-        const int64_t most = (n + least - 1) / least;
-        s = s < most ? s : most;
-        return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-    };
+    const int64_t TG = (int64_t)T * (H / Hkv), all = (int64_t)B * H * T;
+    const double step = D * 1.55 / 128, step2 = D * 2.0 / 128, kstep = D * 1.0 / 128;
     if (prefix > 0 && TG < 128 && B > 1) {                    // rows of all requests in one tile: the prefix is read once, not once per request
         const int64_t R = B * TG;
         P.rwp = R <= 32 ? 1 : 4;
         P.rw = TG <= 32 ? 1 : 4;
         P.packed_tiles = (int)((R + 32 * P.rwp - 1) / (32 * P.rwp));
-        P.packed_split = cut((int64_t)Hkv * P.packed_tiles, prefix, P.rwp == 1 ? 128 : 64);
+        P.packed_split = P.rwp == 1 ? att_cut((int64_t)Hkv * P.packed_tiles, prefix, 128, kstep, 2 * kstep, all, D, 1)
+                                    : att_cut((int64_t)Hkv * P.packed_tiles, prefix, 64, step, step2, all, D, 1);
         P.tiles = (int)((TG + 32 * P.rw - 1) / (32 * P.rw));
         P.split = 1;
         P.slots = P.packed_split + 1;
@@ -725,9 +754,11 @@ static AttPlan att_plan(int B, int H, int Hkv, int T, int64_t keys, int64_t pref
     P.rwp = P.rw = TG <= 32 ? 1 : 4;
     const int per = 32 * P.rw;
     P.tiles = (int)((TG + per - 1) / per);
-    P.split = cut((int64_t)B * Hkv * P.tiles, keys + prefix, P.rw == 1 ? 128 : 64);
+    const int64_t items = (int64_t)B * Hkv * P.tiles;
+    P.split = P.rw == 1 ? att_cut(items, keys + prefix, 128, kstep, 2 * kstep, all, D, advance ? 1 : 0)
+                        : att_cut(items, keys + prefix, 64, step, step2, all, D, advance ? 1 : 0);
     P.slots = P.split > 1 || advance ? P.split : 0;
-    P.blocks = (int64_t)B * Hkv * P.tiles * P.split;
+    P.blocks = items * P.split;
     return P;
 }
 
@@ -757,14 +788,18 @@ static int att_launch(AttendArgs &A, const AttPlan &P, int advance, int32_t *len
     if (!A.slots) return FASTKV_OK;
     const int64_t nrows = (int64_t)A.B * A.H * A.T;
     ProfScope ps_(K_ATTEND, st);
-    hipLaunchKernelGGL((attend_join_kernel<D, BF>), dim3((unsigned)((nrows + 3) / 4)), dim3(256), 0, st, A, nrows, advance ? A.T : 0, len,
-                       advance ? abort_flag_device() : nullptr);
+    const bool many = A.slots >= 8;
+    const int per = many ? 256 / (D * 2) + (D == 256) : 1024 / D;
+    const dim3 grid((unsigned)((nrows + per - 1) / per)), block(256);
+    uint32_t *flag = advance ? abort_flag_device() : nullptr;
+    if (many) hipLaunchKernelGGL((attend_join_kernel<D, BF, D == 256 ? 4 : 8>), grid, block, 0, st, A, nrows, advance ? A.T : 0, len, flag);
+    else hipLaunchKernelGGL((attend_join_kernel<D, BF, 1>), grid, block, 0, st, A, nrows, advance ? A.T : 0, len, flag);
     return hipGetLastError() == hipSuccess ? FASTKV_OK : FASTKV_ELAUNCH;
 }
 
 static int att_run(AttendArgs &A, int dtype, int D, int64_t keys, int advance, int32_t *len, void *workspace, size_t workspace_bytes, void *stream)
 {
-    const AttPlan P = att_plan(A.B, A.H, A.Hkv, A.T, keys, A.prefix, advance != 0);
+    const AttPlan P = att_plan(A.B, A.H, A.Hkv, D, A.T, keys, A.prefix, advance != 0);
     if (P.blocks > 0x7fffffff) return FASTKV_EUNSUPPORTED;
     const size_t need = att_bytes(P, A.B, A.H, A.T, D);
     if (need && (!workspace || ((uintptr_t)workspace & 15))) return FASTKV_EINVAL;
@@ -814,7 +849,7 @@ size_t fastkv_attend_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t 
                                      int32_t prefix, int32_t advance)
 {
     if (!att_shape_ok(FASTKV_F16, B, H, Hkv, D, T, rows) || window < 0 || sinks < 0 || prefix < 0) return 0;
-    return att_bytes(att_plan(B, H, Hkv, T, att_keys(T, rows, window ? window : rows, sinks), prefix, advance != 0), B, H, T, D);
+    return att_bytes(att_plan(B, H, Hkv, D, T, att_keys(T, rows, window ? window : rows, sinks), prefix, advance != 0), B, H, T, D);
 }
 
 int fastkv_window_attention(int32_t dtype, int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t T, const void *q, const int64_t q_strides[3],
