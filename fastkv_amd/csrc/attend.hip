@@ -720,10 +720,10 @@ struct AttPlan { int rwp, rw, packed_tiles, packed_split, tiles, split, slots; i
 static int att_cut(int64_t items, int64_t n, int per, double step, double step2, int64_t rows, int D, int extra)
 {
     const int64_t steps = (n + per - 1) / per;
-    const int most = (int)(steps < 64 ? steps : 64);
     int best = 1;
     double least = 1e30;
-    for (int s = 1; s <= most; ++s) {
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+        if (s > steps) break;
         const int64_t wgs = items * s, each = (steps + s - 1) / s;
         const int64_t full = wgs / 512, rest = wgs % 512;
         double t = (double)(full * (2.5 + each * step2)) + (rest ? 2.5 + each * (rest > 256 ? step2 : step) : 0.0);

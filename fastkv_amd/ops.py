@@ -6,6 +6,7 @@ All functions are stream-ordered on torch's current stream and never synchronise
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional, Tuple
 
@@ -486,6 +487,12 @@ def _launch(what, index, fn, *args) -> None:
         check(rc, what)
 
 
+@functools.lru_cache(maxsize=1024)
+def _attend_bytes(*shape) -> int:
+    # (how a call is cut depends on its shape alone)
+    return load().fastkv_attend_workspace_bytes(*shape)
+
+
 def _attend(what, q, k, v, len_dev, window, sinks, scaling, advance, k_prefix=None, v_prefix=None):
     """The checks, output, scratch and call of the three attention forms.  Output and scratch come from the caching allocator in every call:
     nothing is kept between calls, so calls on several streams and captured graphs (whose scratch lives in their own pool) cannot meet
@@ -516,27 +523,26 @@ def _attend(what, q, k, v, len_dev, window, sinks, scaling, advance, k_prefix=No
         length, step = len_dev.data_ptr(), 1 if len_dev.shape[0] > 1 else 0
     P = 0
     if k_prefix is not None:
-        if k_prefix.dim() == 4 and k_prefix.shape[0] == 1 and v_prefix.dim() == 4 and v_prefix.shape[0] == 1:
-            k_prefix, v_prefix = k_prefix[0], v_prefix[0]
         if k_prefix.dtype is not dtype or v_prefix.dtype is not dtype:
             raise TypeError(f"fastkv_amd.{what}: q, k and v must have one type")
-        if k_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape or k_prefix.shape[0] != Hkv or k_prefix.shape[2] != D or k_prefix.shape[1] == 0 \
-                or k_prefix.stride(2) != 1 or v_prefix.stride(2) != 1:
-            raise ValueError(f"fastkv_amd.{what}: expected prefixes [{Hkv},P >= 1,{D}] with unit head_dim stride, got {tuple(k_prefix.shape)}, "
+        pshape, kps, vps = k_prefix.shape, k_prefix.stride(), v_prefix.stride()
+        if pshape != v_prefix.shape or len(pshape) not in (3, 4) or pshape[:-3] not in ((), (1,)) or pshape[-3] != Hkv or pshape[-1] != D \
+                or pshape[-2] == 0 or kps[-1] != 1 or vps[-1] != 1:
+            raise ValueError(f"fastkv_amd.{what}: expected prefixes [{Hkv},P >= 1,{D}] with unit head_dim stride, got {tuple(pshape)}, "
                              f"{tuple(v_prefix.shape)}")
-        P = k_prefix.shape[1]
+        P = pshape[-2]
     dev = q.device
     out = torch.empty((B, T, H * D), dtype=dtype, device=dev)
     if out.numel() == 0:
         return out
     lib = load()
     adv = 1 if advance else 0
-    need = lib.fastkv_attend_workspace_bytes(B, H, Hkv, D, T, rows, window, sinks, P, adv)
+    need = _attend_bytes(B, H, Hkv, D, T, rows, window, sinks, P, adv)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     wp = ws.data_ptr() if need else None
     if P:
         _launch(what, index, lib.fastkv_shared_prefix_attention, code, B, H, Hkv, D, T, q.data_ptr(), _S4(*qs), k_prefix.data_ptr(),
-                _S3(*k_prefix.stride()), v_prefix.data_ptr(), _S3(*v_prefix.stride()), P, k.data_ptr(), _S4(*ks), v.data_ptr(), _S4(*vs), rows,
+                _S3(*kps[-3:]), v_prefix.data_ptr(), _S3(*vps[-3:]), P, k.data_ptr(), _S4(*ks), v.data_ptr(), _S4(*vs), rows,
                 length, step, adv, scaling, out.data_ptr(), wp, need)
     else:
         _launch(what, index, lib.fastkv_window_attention, code, B, H, Hkv, D, T, q.data_ptr(), _S4(*qs), k.data_ptr(), _S4(*ks), v.data_ptr(),
@@ -591,9 +597,13 @@ def decode_shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_pr
 def _per_row(t, dtype, B, what, name):
     if t is None:
         return None, 0
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] not in (1, B) or not t.is_contiguous():
-        raise ValueError(f"fastkv_amd.{what}: {name} must be a contiguous {dtype} tensor of 1 or {B} values")
-    return t.data_ptr(), 1 if t.shape[0] > 1 else 0
+    if t.dtype is dtype and t.dim() == 1:
+        n = t.shape[0]
+        if n == 1:
+            return t.data_ptr(), 0
+        if n == B and t.stride(0) == 1:
+            return t.data_ptr(), 1
+    raise ValueError(f"fastkv_amd.{what}: {name} must be a contiguous {dtype} tensor of 1 or {B} values")
 
 
 def _row_table(t, dtype, B, width, what, name):
