@@ -32,12 +32,27 @@ def _window_allows_static(config, past_key_values) -> bool:
     """The HIP decode attention attends over ALL rows of the slab (no mask: one new token sees the whole cache).  A model with a
     sliding window (Mistral v0.1: `config.sliding_window`) limits attention to the last `window` positions in the eager path
     (mistral_model.py passes the window to the mask builder and the attention call): the two agree only while the slabs cannot
-    hold more rows than the window.  Otherwise static decode is refused up front instead of diverging silently."""
+    hold more rows than the window.  Otherwise the step's attention is `ops.decode_window_attention` (see `_static_window`)."""
     win = getattr(config, "sliding_window", None)
     if win is None:
         return True
     layers = getattr(past_key_values, "layers", None) or []
     return all(getattr(l, "kslab", None) is None or l.kslab.shape[2] <= win for l in layers)
+
+
+def _static_window(config, slab):
+    """The window that a static step's attention over this slab has to keep to, None if the slab cannot outgrow it (then the dense decode
+    kernels see the same rows): rows j > len - window of the slab, as the eager path's mask has them."""
+    win = getattr(config, "sliding_window", None)
+    return win if win is not None and slab.kslab.shape[2] > win else None
+
+
+def _prefill_window(config, query_states) -> bool:
+    """FASTKV_WINDOW_ATTENTION=1: the prefill attention of a model with a sliding window runs through `ops.window_attention` instead of SDPA
+    with a dense mask (unpadded prompts, as everything here)."""
+    return os.environ.get("FASTKV_WINDOW_ATTENTION", "0") == "1" and getattr(config, "sliding_window", None) is not None \
+        and query_states.is_cuda and query_states.dtype in (torch.float16, torch.bfloat16) and query_states.shape[-1] in (64, 128, 256) \
+        and not (torch.is_grad_enabled() and query_states.requires_grad)
 
 
 def _norm(module, hidden_states, static):
@@ -88,6 +103,8 @@ def _static_layer_ok(layer, hidden_states, position_embeddings, past_key_values)
     layers = getattr(past_key_values, "layers", None)
     slab = layers[attn.layer_idx] if layers is not None and attn.layer_idx < len(layers) else None
     if not (isinstance(slab, SlabLayer) and slab.static_decode) or position_embeddings[0].dtype != torch.float16:
+        return False
+    if _static_window(attn.config, slab) is not None:             # (the one-launch attention of the step sees every row)
         return False
     if not all(hasattr(m, "variance_epsilon") and m.weight.dtype == torch.float16
                for m in (layer.input_layernorm, layer.post_attention_layernorm)):
@@ -204,10 +221,18 @@ def make_attention_class(base_cls, modeling, extra_attn_kwargs):
                         # static decode over the slab: append + GQA attention through the HIP decode kernels, the length is a
                         # device-side counter -> no shape changes, the step is graph-capturable (fastkv_amd/cache.py)
                         ops.decode_append(slab.kslab, slab.vslab, key_states, value_states, slab.len_dev)
-                        attn_output = ops.decode_attention(query_states, slab.kslab, slab.vslab, slab.len_dev, self.scaling, workspace=slab.attn_ws)
+                        win = _static_window(self.config, slab)
+                        if win is None:
+                            attn_output = ops.decode_attention(query_states, slab.kslab, slab.vslab, slab.len_dev, self.scaling, workspace=slab.attn_ws)
+                        else:
+                            attn_output = ops.decode_window_attention(query_states, slab.kslab, slab.vslab, slab.len_dev, self.scaling, window=win)
                         slab.host_step()
                         return self.o_proj(attn_output.view(*input_shape, -1)), None
                     key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)
+
+            if q_len > 1 and key_states.shape[2] == q_len and _prefill_window(self.config, query_states):
+                attn_output = ops.window_attention(query_states, key_states, value_states, window=self.config.sliding_window, scaling=self.scaling)
+                return self.o_proj(attn_output), None
 
             attention_interface = modeling.ALL_ATTENTION_FUNCTIONS.get_interface(self.config._attn_implementation,
                                                                                 modeling.eager_attention_forward)
@@ -361,10 +386,6 @@ def make_model_forward(modeling, mask_fn_for):
         if sp is not None and position_ids is None:
             position_ids = (torch.arange(inputs_embeds.shape[1], device=inputs_embeds.device) + sp.pos0).unsqueeze(0)
             position_ids = position_ids.expand(inputs_embeds.shape[0], -1)
-        if getattr(past_key_values, "static_decode", False) and not _window_allows_static(self.config, past_key_values):
-            raise ValueError(f"static decode attends over the whole cache slab, but this model has sliding_window = "
-                             f"{self.config.sliding_window} and the slabs hold more rows than that: decode eagerly "
-                             "(cache.finish_static_decode()) or size the slabs within the window")
         if position_ids is None:
             if getattr(past_key_values, "static_decode", False):
                 raise ValueError("static decode (graph-capturable) needs position_ids as a device tensor: a host-side position "

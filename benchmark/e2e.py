@@ -26,7 +26,38 @@ import torch
 from benchmark import prefill as P
 
 
-def graph_decode(model, pkv, tok, steps, timed):
+class Penalties:
+    """Repetition / presence / frequency penalties of a run (`--repetition_penalty`, ...): the requests' histories and lengths on the device, and
+    `ops.decode_penalties` in front of the greedy choice.  History, lengths and penalties are tensors, so a captured step replays with them."""
+
+    def __init__(self, args, prompt, genlen):
+        B, L = prompt.shape
+        dev = prompt.device
+        self.tokens = torch.zeros(B, L + genlen + 1, dtype=torch.int64, device=dev)
+        self.tokens[:, :L] = prompt
+        self.n = torch.full((B,), L, dtype=torch.int32, device=dev)
+        self.n_prompt = self.n.clone()
+        self.values = [torch.full((1,), v, dtype=torch.float32, device=dev) if v != off else None for v, off in
+                       ((args.repetition_penalty, 1.0), (args.presence_penalty, 0.0), (args.frequency_penalty, 0.0))]
+
+    @staticmethod
+    def wanted(args) -> bool:
+        if getattr(args, "repetition_penalty", 1.0) <= 0:
+            raise ValueError("--repetition_penalty must be positive")
+        return (getattr(args, "repetition_penalty", 1.0), getattr(args, "presence_penalty", 0.0), getattr(args, "frequency_penalty", 0.0)) != (1.0, 0.0, 0.0)
+
+    def apply(self, logits):
+        """The penalised logits [B,V] of the last position."""
+        from fastkv_amd import ops
+        return ops.decode_penalties(logits[:, -1, :], self.tokens, self.n, self.n_prompt, *self.values)
+
+    def said(self, tok):
+        """tok [B,1] joins the histories."""
+        self.tokens.scatter_(1, self.n.long()[:, None], tok)
+        self.n.add_(1)
+
+
+def graph_decode(model, pkv, tok, steps, timed, penalties=None):
     """`steps` greedy decode steps over a slab cache in static-decode mode: the first one eagerly (it warms every library up on
     this stream and is a real, counted step), then ONE capture of the step and `steps - 1` replays.  Returns (ms, tokens)."""
     dev = tok.device
@@ -48,10 +79,15 @@ def graph_decode(model, pkv, tok, steps, timed):
 
     def step():
         out = model(input_ids=tok_buf, past_key_values=pkv, position_ids=pos_buf)
-        if fused_tail and out.logits.dtype == torch.float16 and out.logits.shape[-1] % 8 == 0:
-            _ops.decode_greedy(out.logits, greedy_scratch, tok_buf, pos_buf, out_tok, step_no)
+        logits = out.logits if penalties is None else penalties.apply(out.logits)[:, None]
+        if fused_tail and logits.dtype == torch.float16 and logits.shape[-1] % 8 == 0:
+            _ops.decode_greedy(logits, greedy_scratch, tok_buf, pos_buf, out_tok, step_no)
+            if penalties is not None:
+                penalties.said(tok_buf)
             return
-        nxt = out.logits[:, -1, :].argmax(dim=-1, keepdim=True)
+        nxt = logits[:, -1, :].argmax(dim=-1, keepdim=True)
+        if penalties is not None:
+            penalties.said(nxt)
         tok_buf.copy_(nxt)
         pos_buf.add_(1)
         out_tok.index_copy_(0, step_no, nxt[0])
@@ -98,6 +134,9 @@ def main(model, args):
         for layer in model.model.layers:
             layer.self_attn.kv_cluster = args.cluster_factory(layer.self_attn.kv_cluster)
     use_events = dev.type == "cuda"
+    penalise = Penalties.wanted(args)
+    if penalise and not use_events:
+        raise ValueError("the penalties run on the GPU only")
 
     def timed(fn):
         if use_events:
@@ -118,20 +157,25 @@ def main(model, args):
         with torch.no_grad():
             t_prefill, out = timed(lambda: model(input_id, attention_mask=attn_mask))
             pkv = out.past_key_values
-            tok = out.logits[:, -1, :].argmax(dim=-1, keepdim=True)
+            penalties = Penalties(args, input_id, args.genlen) if penalise else None
+            tok = (penalties.apply(out.logits) if penalise else out.logits[:, -1, :]).argmax(dim=-1, keepdim=True)
+            if penalise:
+                penalties.said(tok)
             generated = [int(tok[0, 0])]
             t_decode = 0.0
             graph_mode = bool(getattr(args, "decode_graph", True)) and use_events and hasattr(pkv, "enable_static_decode") \
                 and args.genlen > 2
             if graph_mode:
-                t_decode, toks = graph_decode(model, pkv, tok, args.genlen - 1, timed)
+                t_decode, toks = graph_decode(model, pkv, tok, args.genlen - 1, timed, penalties)
                 generated += toks
             else:
                 for _ in range(args.genlen - 1):
                     dt, out = timed(lambda: model(input_ids=tok, past_key_values=pkv))
                     t_decode += dt
                     pkv = out.past_key_values
-                    tok = out.logits[:, -1, :].argmax(dim=-1, keepdim=True)
+                    tok = (penalties.apply(out.logits) if penalise else out.logits[:, -1, :]).argmax(dim=-1, keepdim=True)
+                    if penalise:
+                        penalties.said(tok)
                     generated.append(int(tok[0, 0]))
         if it >= args.num_warmups:
             results.append((t_prefill, t_decode, len(generated)))

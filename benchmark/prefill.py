@@ -159,6 +159,9 @@ def parse_args(argv=None):
     p.add_argument("--genlen", type=int, default=128)
     p.add_argument("--decode_graph", type=int, default=1, help="e2e.py on the GPU with FASTKV_SLAB_CACHE=1: capture the decode "
                                                              "step in a HIP graph (HIP decode attention over the slab cache)")
+    p.add_argument("--repetition_penalty", type=float, default=1.0, help="e2e.py: penalties on the tokens of prompt and answer, in front of the greedy choice")
+    p.add_argument("--presence_penalty", type=float, default=0.0)
+    p.add_argument("--frequency_penalty", type=float, default=0.0)
     p.add_argument("--num_warmups", type=int, default=1)
     p.add_argument("--num_runs", type=int, default=1)
     p.add_argument("--eval_batch_size", type=int, default=1)
