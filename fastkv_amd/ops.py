@@ -467,13 +467,14 @@ _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda ind
 
 def _on_device(what: str, index: int, tensors) -> None:
     # (kernels are launched on that device's current stream; nothing here has a backward pass, and none is faked)
-    grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is not None:
-            if t.get_device() != index or index < 0:
+        if t is not None and (t.get_device() != index or t.requires_grad):
+            if index < 0 or t.get_device() != index:
                 raise RuntimeError(f"fastkv_amd.{what}: all tensors must be on one ROCm device (no CPU fallback exists)")
-            if grad and t.requires_grad:
+            if torch.is_grad_enabled():
                 raise RuntimeError(f"fastkv_amd.{what} has no backward pass: call it under torch.no_grad()")
+    if index < 0:
+        raise RuntimeError(f"fastkv_amd.{what}: all tensors must be on one ROCm device (no CPU fallback exists)")
 
 
 def _launch(what, index, fn, *args) -> None:
@@ -594,7 +595,8 @@ def decode_shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_pr
     return _attend(what, q, kslab, vslab, len_dev, 0, 0, scaling, advance, k_prefix, v_prefix)
 
 
-def _per_row(t, dtype, B, what, name):
+def _per_row(t, dtype, B, name):
+    # (address, step) of one value per row or one for all
     if t is None:
         return None, 0
     if t.dtype is dtype and t.dim() == 1:
@@ -603,16 +605,17 @@ def _per_row(t, dtype, B, what, name):
             return t.data_ptr(), 0
         if n == B and t.stride(0) == 1:
             return t.data_ptr(), 1
-    raise ValueError(f"fastkv_amd.{what}: {name} must be a contiguous {dtype} tensor of 1 or {B} values")
+    raise ValueError(f"fastkv_amd.decode_penalties: {name} must be a contiguous {dtype} tensor of 1 or {B} values")
 
 
-def _row_table(t, dtype, B, width, what, name):
+def _row_table(t, dtype, B, width, name):
+    # (address, row stride) of one row per row or one for all
     if t is None:
         return None, 0
-    if t.dtype is not dtype or t.dim() not in (1, 2) or t.shape[-1] != width or (t.dim() == 2 and t.shape[0] not in (1, B)) \
-            or (width > 1 and t.stride(-1) != 1):
-        raise ValueError(f"fastkv_amd.{what}: {name} must be {dtype} [{width}], [1,{width}] or [{B},{width}] with unit stride")
-    return t.data_ptr(), t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else 0
+    shape = t.shape
+    if t.dtype is dtype and (len(shape) == 1 or (len(shape) == 2 and shape[0] in (1, B))) and shape[-1] == width and (width == 1 or t.stride(-1) == 1):
+        return t.data_ptr(), t.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
+    raise ValueError(f"fastkv_amd.decode_penalties: {name} must be {dtype} [{width}], [1,{width}] or [{B},{width}] with unit stride")
 
 
 def decode_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, n_tokens: Optional[torch.Tensor] = None,
@@ -651,10 +654,10 @@ def decode_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None
     if B == 0:
         return out
     _launch(what, index, load().fastkv_decode_penalties, code, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, tp, ts, L,
-            *_per_row(n_tokens, torch.int32, B, what, "n_tokens"), *_per_row(n_prompt, torch.int32, B, what, "n_prompt"),
-            *_per_row(repetition, torch.float32, B, what, "repetition"), *_per_row(presence, torch.float32, B, what, "presence"),
-            *_per_row(frequency, torch.float32, B, what, "frequency"), *_row_table(bias, torch.float32, B, V, what, "bias"),
-            *_row_table(allowed, torch.int32, B, (V + 31) // 32, what, "allowed"), out.data_ptr(), out.stride(0) if B > 1 else V)
+            *_per_row(n_tokens, torch.int32, B, "n_tokens"), *_per_row(n_prompt, torch.int32, B, "n_prompt"),
+            *_per_row(repetition, torch.float32, B, "repetition"), *_per_row(presence, torch.float32, B, "presence"),
+            *_per_row(frequency, torch.float32, B, "frequency"), *_row_table(bias, torch.float32, B, V, "bias"),
+            *_row_table(allowed, torch.int32, B, (V + 31) // 32, "allowed"), out.data_ptr(), out.stride(0) if B > 1 else V)
     return out
 
 
