@@ -209,7 +209,8 @@ template <int D, int NB, int NW> struct AttLoad {
     // last key -- their scores are cut off, but a V row there must be finite.
     template <bool V> static __device__ __forceinline__ void any(const AttKeys &K, int u0, uint16_t *dst, int w)
     {
-        const int lane = threadIdx.x & 63;
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));           // (nothing of this is worth registers across the loop)
         const uint32_t lds = lds_of(dst, w);
         att_each<0, CH>([&](auto I) {
             constexpr int i = I;
@@ -423,8 +424,9 @@ template <int RWP, int RW> __device__ __forceinline__ AttItem att_item(const Att
     return it;
 }
 
-// an item, by four waves.  RW = 4: rows, RW = 1: keys (see above)
-template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(const AttendArgs &A, const AttItem &it, uint16_t *smem)
+// An item, by four waves.  RW = 4: rows, RW = 1: keys (see above).  SAME: all rows see the same keys (one token per request, the prefix of a batch);
+// what partly seen tiles need would cost a single token its registers at 256 dims (1.5 TB/s of the caches instead of 4.8).
+template <int D, bool BF, int RW, bool SAME> __device__ __forceinline__ void att_item_body(const AttendArgs &A, const AttItem &it, uint16_t *smem)
 {
     constexpr int NB = RW == 4 ? 2 : 1, KT = 32 * NB, KW = 4 / RW;
     constexpr int TILE = KT * D;                             // elements of a K (or V) tile
@@ -501,7 +503,7 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
         __syncthreads();
         att_landed<0>();
         bool lean = K.lean(u_lo);
-        if (u_lo < K.N && !lean) Load::template scan<BF>(smem + TILE, w, &s_wild[0]);
+        if (!SAME && u_lo < K.N && !lean) Load::template scan<BF>(smem + TILE, w, &s_wild[0]);
         __syncthreads();
         int at = 0, wl = 0;                                   // the tile's place in shared memory, its word of s_wild
         for (int u = u_lo; u < K.N; u += KT) {
@@ -522,11 +524,11 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
                 att_scores<D, BF, NB>(cur, Q, S);
                 att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, !lean);
                 att_values<D, BF, NB>(cur + TILE, P, O);
-                if (!lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, s_wild[wl]);
+                if (!SAME && !lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, s_wild[wl]);
             }
             att_landed<0>();
-            if (more && !next_lean) Load::template scan<BF>(nxt + TILE, w, &s_wild[wn]);     // (a lane looks at what it brought itself)
-            if (tid == 0) s_wild[wn == 2 ? 0 : wn + 1] = 0;  // last read a tile ago, written a tile from now
+            if (!SAME && more && !next_lean) Load::template scan<BF>(nxt + TILE, w, &s_wild[wn]);      // (a lane looks at what it brought itself)
+            if (!SAME && tid == 0) s_wild[wn == 2 ? 0 : wn + 1] = 0;     // last read a tile ago, written a tile from now
             __syncthreads();
             at ^= 2 * TILE;
             wl = wn;
@@ -553,7 +555,7 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
             if (next_whole) att_landed<Load::CH>();
             else att_landed<0>();
             uint64_t wild = 0;
-            if (!lean && p_lo != p_hi) {                     // (rows at one position see the same keys)
+            if (!SAME && !lean) {
                 if (lane == 0) s_wild[w] = 0;
                 asm volatile("" ::: "memory");
                 Load::template scan<BF>(vs, 0, &s_wild[w]);  // (one wave's accesses to shared memory are in order)
@@ -561,7 +563,7 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
                 wild = s_wild[w];
             }
             att_values<D, BF, NB>(vs, P, O);
-            if (!lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, wild);
+            if (!SAME && !lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, wild);
             att_read_done();
             if (more) Load::template issue<true>(K, un, vs, 0);
             u = un;
@@ -638,14 +640,14 @@ template <int D, bool BF, int RW> __device__ __forceinline__ void att_item_body(
 }
 
 // RWP: shape of the items over all requests' rows (a shared prefix), RW: of the others
-template <int D, bool BF, int RWP, int RW>
+template <int D, bool BF, int RWP, int RW, bool ONE>
 __global__ void __launch_bounds__(ATT_THREADS, D <= 128 ? 2 : 1) attend_kernel(const AttendArgs A)
 {
     __shared__ __attribute__((aligned(16))) uint16_t smem[256 * D + 1024];         // tiles: 256 rows of D; the joined rows: 4 * 32 * (D + 4) floats
     const AttItem it = att_item<RWP, RW>(A);
-    if (RWP == RW) att_item_body<D, BF, RW>(A, it, smem);
-    else if (it.packed) att_item_body<D, BF, RWP>(A, it, smem);
-    else att_item_body<D, BF, RW>(A, it, smem);
+    if (RWP == RW) att_item_body<D, BF, RW, ONE>(A, it, smem);
+    else if (it.packed) att_item_body<D, BF, RWP, true>(A, it, smem);
+    else att_item_body<D, BF, RW, ONE>(A, it, smem);
 }
 
 // The slices of a row, joined: out = sum 2^(c (m_i - M)) O_i / sum 2^(c (m_i - M)) l_i.  A thread has four dims of a row; SG threads share the
@@ -737,11 +739,12 @@ static AttPlan att_plan(int B, int H, int Hkv, int D, int T, int64_t keys, int64
 {
     AttPlan P = {};
     const int64_t TG = (int64_t)T * (H / Hkv), all = (int64_t)B * H * T;
+    const int few = T == 1 || D < 256 ? 32 : 0;               // rows up to which the keys shape is taken
     const double step = D * 1.55 / 128, step2 = D * 2.0 / 128, kstep = D * 1.0 / 128;
     if (prefix > 0 && TG < 128 && B > 1) {                    // rows of all requests in one tile: the prefix is read once, not once per request
         const int64_t R = B * TG;
-        P.rwp = R <= 32 ? 1 : 4;
-        P.rw = TG <= 32 ? 1 : 4;
+        P.rwp = R <= few ? 1 : 4;
+        P.rw = TG <= few ? 1 : 4;
         P.packed_tiles = (int)((R + 32 * P.rwp - 1) / (32 * P.rwp));
         P.packed_split = P.rwp == 1 ? att_cut((int64_t)Hkv * P.packed_tiles, prefix, 128, kstep, 2 * kstep, all, D, 1)
                                     : att_cut((int64_t)Hkv * P.packed_tiles, prefix, 64, step, step2, all, D, 1);
@@ -751,7 +754,7 @@ static AttPlan att_plan(int B, int H, int Hkv, int D, int T, int64_t keys, int64
         P.blocks = (int64_t)Hkv * P.packed_tiles * P.packed_split + (int64_t)B * Hkv * P.tiles;
         return P;
     }
-    P.rwp = P.rw = TG <= 32 ? 1 : 4;
+    P.rwp = P.rw = TG <= few ? 1 : 4;
     const int per = 32 * P.rw;
     P.tiles = (int)((TG + per - 1) / per);
     const int64_t items = (int64_t)B * Hkv * P.tiles;
@@ -780,9 +783,12 @@ static int att_launch(AttendArgs &A, const AttPlan &P, int advance, int32_t *len
     {
         ProfScope ps_(K_ATTEND, st);
         const dim3 grid((unsigned)P.blocks), block(ATT_THREADS);
-        if (P.rwp == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 1, 1>), grid, block, 0, st, A);
-        else if (P.rw == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 4, 1>), grid, block, 0, st, A);
-        else hipLaunchKernelGGL((attend_kernel<D, BF, 4, 4>), grid, block, 0, st, A);
+        constexpr bool SEVERAL = D == 256;                    // (no keys shape for several tokens of 256 dims: att_plan)
+        if (P.rwp == 1 && A.T == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 1, 1, true>), grid, block, 0, st, A);
+        else if (P.rwp == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 1, 1, SEVERAL>), grid, block, 0, st, A);
+        else if (P.rw == 1 && A.T == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 4, 1, true>), grid, block, 0, st, A);
+        else if (P.rw == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 4, 1, SEVERAL>), grid, block, 0, st, A);
+        else hipLaunchKernelGGL((attend_kernel<D, BF, 4, 4, false>), grid, block, 0, st, A);
     }
     if (hipGetLastError() != hipSuccess) return FASTKV_ELAUNCH;
     if (!A.slots) return FASTKV_OK;
@@ -800,7 +806,7 @@ static int att_launch(AttendArgs &A, const AttPlan &P, int advance, int32_t *len
 static int att_run(AttendArgs &A, int dtype, int D, int64_t keys, int advance, int32_t *len, void *workspace, size_t workspace_bytes, void *stream)
 {
     const AttPlan P = att_plan(A.B, A.H, A.Hkv, D, A.T, keys, A.prefix, advance != 0);
-    if (P.blocks > 0x7fffffff) return FASTKV_EUNSUPPORTED;
+    if (P.blocks > 0xffffff || (int64_t)A.B * A.H * A.T > 0xffffff) return FASTKV_EUNSUPPORTED;      // (a launch of less than 2^32 threads)
     const size_t need = att_bytes(P, A.B, A.H, A.T, D);
     if (need && (!workspace || ((uintptr_t)workspace & 15))) return FASTKV_EINVAL;
     if (workspace_bytes < need) return FASTKV_EWORKSPACE;
@@ -824,7 +830,7 @@ static int att_run(AttendArgs &A, int dtype, int D, int64_t keys, int advance, i
 static bool att_shape_ok(int dtype, int B, int H, int Hkv, int D, int T, int rows)
 {
     return (dtype == FASTKV_F16 || dtype == FASTKV_BF16) && B >= 1 && Hkv >= 1 && H >= Hkv && H % Hkv == 0 && T >= 1 && rows >= 1 &&
-           (int64_t)B * H * T <= 0x7fffffff && rows <= 0x3fffffff && D >= 1;
+           (int64_t)B * H * T <= 0x7fffffff && rows <= 0x1fffffff && D >= 1;
 }
 // 16-byte rows of [n0,n1,n2] or [n1,n2]; along an extent of one nothing is stepped, whatever stride the caller has for it: it becomes 0 in `to`
 static bool att_rows_ok(const void *p, const int64_t *s, std::initializer_list<int> extents, std::initializer_list<int64_t *> to)
@@ -886,7 +892,7 @@ int fastkv_shared_prefix_attention(int32_t dtype, int32_t B, int32_t H, int32_t 
                                    int32_t rows, int32_t *len_dev, int32_t len_step, int32_t advance, float scaling, void *out, void *workspace,
                                    size_t workspace_bytes, void *stream)
 {
-    if (!att_shape_ok(dtype, B, H, Hkv, D, T, rows) || prefix_rows < 1 || prefix_rows > 0x3fffffff) return FASTKV_EINVAL;
+    if (!att_shape_ok(dtype, B, H, Hkv, D, T, rows) || prefix_rows < 1 || prefix_rows > 0x1fffffff) return FASTKV_EINVAL;
     if (D != 64 && D != 128 && D != 256) return FASTKV_EUNSUPPORTED;
     AttendArgs A = {};
     if (!att_rows_ok(q, q_strides, {B, H, T}, {&A.q_b, &A.q_h, &A.q_t}) || !att_rows_ok(k, k_strides, {B, Hkv, rows}, {&A.k_b, &A.k_h, &A.k_r}) ||
