@@ -19,10 +19,24 @@
 // of the request's cache.  Work is cut along u, so a window that starts far behind its sinks costs no empty tiles.
 //
 // Two shapes of a workgroup (4 waves):
-//   rows      4 x 32 rows, all waves on one 64-key tile (two tiles in shared memory, one barrier per tile)
+//   rows      4 x 32 rows, all waves on one 64-key tile (two tiles in shared memory, one barrier per tile); two workgroups per compute unit, whose
+//             products and exponentials fall beside each other as they drift apart
 //   keys      <= 32 rows (single tokens): each wave has its own 32-key tiles and running state, merged at the end; a wave's tile is
 //             private, so the loop has no barrier and eight waves of a compute unit keep ~128 KB of loads in flight
+// Tiles go from memory to shared memory without passing registers (a wave has 512 / 2 of them at 128 dims, all in use).
 // Work too small to fill the chip is cut along the keys; slices leave {m, l, O} in a workspace and attend_join adds them up.
+//
+// What bounds it, measured (H 32, Hkv 8, D 128):
+//   prompts   the matrix pipe, the vector pipe and the clock together: 8k tokens, window 4096: 0.44 ms, 940 TFLOP/s (an 8192^3 library product:
+//             1110); 32k: 2.18 ms, 950.  Per tile of a wave 1024 cycles of products beside ~1000 of vector work; the clock falls to
+//             1.95 GHz under it.  Leaving out the exponentials / the loads / the second product gives 7 / 14 / 12 %: nothing alone bounds it.
+//             Slower: two groups of waves held half a tile apart by barriers (0.53 ms), raised wave priorities (+3 %), exponentials
+//             interleaved with products by hand (+3 %), 32-key tiles (registers spill at three waves per SIMD).
+//   tokens    the memory: 32 requests, window 4096: 88 us, 5.4 TB/s of K and V (a large copy: 5.1 read + write); one request, window 2048:
+//             7.3 + 3.9 us, the latency of the chain kernel arguments - length - K - V - join - second launch
+//   prefix    64 requests on 32768 shared rows: 65 + 9 us: 38 of products (twice 128 rows per KV head), 13 of the requests' own rows, the
+//             slices' sums.  Alternating the shared and the own items over the grid is slower (84): a lone rows-shaped workgroup on a compute unit
+//             has nothing beside its products.
 #include <limits.h>
 #include <initializer_list>
 #include <type_traits>
