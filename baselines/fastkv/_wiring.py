@@ -230,7 +230,7 @@ def make_attention_class(base_cls, modeling, extra_attn_kwargs):
                         return self.o_proj(attn_output.view(*input_shape, -1)), None
                     key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)
 
-            if q_len > 1 and key_states.shape[2] == q_len and _prefill_window(self.config, query_states):
+            if q_len > 1 and key_states.shape[2] == q_len and not self.training and _prefill_window(self.config, query_states):
                 attn_output = ops.window_attention(query_states, key_states, value_states, window=self.config.sliding_window, scaling=self.scaling)
                 return self.o_proj(attn_output), None
 

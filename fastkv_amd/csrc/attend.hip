@@ -77,6 +77,7 @@ struct AttendArgs {
     int slots;                               // slices per row; 0: the result goes to `out`
     int packed_tiles, packed_split, slot0;   // shared prefix, few rows per request: row tiles over ALL requests in front of the grid
     int tiles, split;                        // row tiles per request, key slices
+    int run;                                 // neighbouring items that one die gets
     bool near_rows;
 };
 
@@ -396,18 +397,18 @@ __device__ __forceinline__ void att_wild_rows(const att_u4 (&P)[NB * 2], att_f16
 __device__ __forceinline__ int att_len(const AttendArgs &A, int b)
 {
     const int n = A.len ? A.len[(int64_t)b * A.len_step] : A.len_all;
-    return n < A.rows - A.T ? n : A.rows - A.T;              // a full cache: the call's rows are its last ones
+    return max(min(n, A.rows - A.T), -A.T);                  // a full cache: the call's rows are its last ones; idle is idle
 }
 
 // Item of a workgroup: rows [row0, row0 + count) of request b's list (or of all requests' lists, packed) against keys [u_lo, u_hi)
 struct AttItem { int b, hk, row0, slice, slot; bool packed; };
 
-// Neighbouring workgroups go round the chip's eight dies: hand each die a run of neighbouring items, so that the row tiles that read the
+// Neighbouring workgroups go round the chip's eight dies: hand each die runs of `run` neighbouring items, so that the row tiles that read the
 // same K / V meet in one L2 (a permutation of [0, n))
-__device__ __forceinline__ int att_spread(int i, int n)
+__device__ __forceinline__ int att_spread(int i, int n, int run)
 {
-    const int per = n / 8, full = per * 8;
-    return i < full ? (i & 7) * per + (i >> 3) : i;
+    const int full = n / (8 * run) * (8 * run), j = i >> 3;
+    return i < full ? (j / run * 8 + (i & 7)) * run + j % run : i;
 }
 
 template <int RWP, int RW> __device__ __forceinline__ AttItem att_item(const AttendArgs &A)
@@ -417,7 +418,7 @@ template <int RWP, int RW> __device__ __forceinline__ AttItem att_item(const Att
     const int np = A.packed_tiles * A.packed_split * A.Hkv;
     it.packed = i < np;
     if (it.packed) {                                         // (tile fastest: the tiles of one slice share its keys)
-        i = att_spread(i, np);
+        i = att_spread(i, np, max(1, np / 8));
         it.row0 = i % A.packed_tiles * (32 * RWP);
         i /= A.packed_tiles;
         it.slice = i % A.packed_split;
@@ -426,7 +427,7 @@ template <int RWP, int RW> __device__ __forceinline__ AttItem att_item(const Att
         it.slot = it.slice;
         return it;
     }
-    i = att_spread(i - np, gridDim.x - np);
+    i = att_spread(i - np, gridDim.x - np, A.run);
     const int tile = i % A.tiles;
     i /= A.tiles;
     it.row0 = (A.tiles - 1 - tile) * (32 * RW);              // the tiles that see most first
@@ -811,7 +812,7 @@ static int att_launch(AttendArgs &A, const AttPlan &P, int advance, int32_t *len
     const bool many = A.slots >= 8;
     const int per = many ? 256 / (D * 2) + (D == 256) : 1024 / D;
     const dim3 grid((unsigned)((nrows + per - 1) / per)), block(256);
-    uint32_t *flag = advance ? abort_flag_device() : nullptr;
+    uint32_t *flag = advance ? abort_flag_device(st) : nullptr;
     if (many) hipLaunchKernelGGL((attend_join_kernel<D, BF, D == 256 ? 4 : 8>), grid, block, 0, st, A, nrows, advance ? A.T : 0, len, flag);
     else hipLaunchKernelGGL((attend_join_kernel<D, BF, 1>), grid, block, 0, st, A, nrows, advance ? A.T : 0, len, flag);
     return hipGetLastError() == hipSuccess ? FASTKV_OK : FASTKV_ELAUNCH;
@@ -831,6 +832,10 @@ static int att_run(AttendArgs &A, int dtype, int D, int64_t keys, int advance, i
     A.slot0 = P.packed_split;
     A.tiles = P.tiles;
     A.split = P.split;
+    // One run per die where the KV heads divide over the dies.  Elsewhere a run would hold the row tiles that see most and another those that see
+    // least (8192 tokens without a window, 16 heads on 2: 452 us so, 331 in runs of four; 8 on 1: 255 and 227).
+    const int64_t own = P.blocks - (int64_t)A.Hkv * P.packed_tiles * P.packed_split;
+    A.run = (int64_t)A.B * A.Hkv % 8 == 0 || own < 64 ? (int)(own / 8 > 1 ? own / 8 : 1) : 4;
     A.near_rows = true;
     for (int64_t r : {A.k_r, A.v_r, A.k0_r, A.v0_r}) A.near_rows = A.near_rows && r >= 0 && r < (int64_t)1 << 23;
     A.part_o = (float *)workspace;

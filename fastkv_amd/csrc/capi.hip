@@ -31,6 +31,13 @@ uint32_t *abort_flag_device()
     });
     return g_abort_dev;
 }
+uint32_t *abort_flag_device(hipStream_t st)
+{
+    if (g_abort_dev) return g_abort_dev;
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &cs) != hipSuccess) (void)hipGetLastError();
+    return cs == hipStreamCaptureStatusNone ? abort_flag_device() : nullptr;
+}
 uint64_t spin_limit_ticks()
 {
     static const uint64_t ticks = []() {

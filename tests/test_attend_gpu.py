@@ -323,3 +323,108 @@ def test_on_another_stream_than_the_tensors():
     here = [ops.decode_window_attention(q, k, v, n, 0.1, window=900, sinks=4, advance=False) for _ in range(8)]
     torch.cuda.synchronize()
     assert all(torch.equal(want, x) for x in got + here)
+
+
+def test_idle_lengths_strides_of_single_extents_and_many_heads_per_kv_head():
+    from fastkv_amd import ops
+    q, k, v = make(2, 3, 4, 2, 64, 2, 30, F16)
+    lens = [-2 ** 31, 7, 2 ** 31 - 1]                               # idle for good, in use, beyond the cache
+    got = ops.window_attention(q.cuda(), k.cuda(), v.cuda(), window=5, sinks=1, len_dev=dev_lens(lens))
+    ref, bound = attend(q, window_rows(k.double(), v.double(), [-2, 7, 28], 2, 5, 1, 2, 4), 64 ** -0.5)
+    check(got, ref, bound)
+    # extents of one may have any stride
+    one = torch.randn(64, dtype=F16, device="cuda").as_strided((1, 1, 1, 64), (3, 5, 7, 1))
+    assert torch.equal(ops.window_attention(one, one, one)[0, 0], one[0, 0, 0])
+    # 40 query heads on one KV head: two row tiles for a single token
+    q, k, v = make(3, 2, 40, 1, 128, 1, 90, BF16)
+    got = ops.decode_window_attention(q.cuda(), k.cuda(), v.cuda(), dev_lens([89, 30]), 0.09, window=33, sinks=2, advance=False)
+    ref, bound = attend(q, window_rows(k.double(), v.double(), [89, 30], 1, 33, 2, 1, 40), 0.09)
+    check(got, ref, bound)
+
+
+@pytest.mark.parametrize("H,Hkv,window", [(6, 3, None), (8, 1, None), (8, 8, 150)])
+def test_longer_prompts_against_sdpa_in_fp32(H, Hkv, window):
+    """Enough row tiles for every die, in runs or whole heads: each row of the output is where it belongs."""
+    from fastkv_amd import ops
+    T, D = 2111, 64
+    q, k, v = (t.cuda() for t in make(H, 1, H, Hkv, D, T, T, F16))
+    got = ops.window_attention(q, k, v, window=window, sinks=2).float().view(T, H, D)
+    kk, vv = (t.float().repeat_interleave(H // Hkv, 1)[0] for t in (k, v))
+    i, j = torch.arange(T, device="cuda")[:, None], torch.arange(T, device="cuda")[None]
+    ok = (j <= i) & ((j < 2) | (j > i - (window or T)))
+    s = (q[0].float() @ kk.transpose(-1, -2).contiguous()) * D ** -0.5
+    want = (torch.softmax(s.masked_fill(~ok, -float("inf")), -1) @ vv).transpose(0, 1)
+    A = 4.0                                                          # sum p |v| of standard normal v is at most a few
+    assert float((got - want).abs().max()) <= 2 ** -10 * A
+
+
+def test_prefix_inside_a_longer_slab_of_another_batch():
+    """The prefix as a view of a cache slab (rows of another stride than the requests' own), for few and for many rows per request."""
+    from fastkv_amd import ops
+    H, Hkv, D, P = 8, 2, 128, 170
+    slab_k, slab_v = (torch.full((1, Hkv, 300, D + 64), float("nan"), dtype=F16) for _ in range(2))
+    for T in (1, 5, 60):
+        q, k, v = make(T, 2, H, Hkv, D, T, 80, F16)
+        _, kp, vp = make(T + 1, 1, H, Hkv, D, 1, P, F16)
+        slab_k[:, :, 20:20 + P, :D], slab_v[:, :, 20:20 + P, :D] = kp, vp
+        sk, sv = slab_k.cuda(), slab_v.cuda()
+        got = ops.decode_shared_prefix_attention(q.cuda(), sk[:, :, 20:20 + P, :D], sv[0, :, 20:20 + P, :D][None], k.cuda(), v.cuda(), dev_lens([3, 20]), 0.1,
+                                                 advance=False)
+        ref, bound = attend(q, prefix_rows(kp[0].double(), vp[0].double(), k.double(), v.double(), [3, 20], T, Hkv, H), 0.1)
+        check(got, ref, bound)
+
+
+def test_together_as_a_step_uses_them_captured():
+    """One document, four requests: the questions' own prefill, then captured single-token steps -- append, attention over prefix and own rows, penalties,
+    greedy choice -- against the same steps run eagerly."""
+    from fastkv_amd import ops
+    B, H, Hkv, D, P, rows, T, V, steps = 4, 8, 2, 64, 300, 64, 9, 512, 6
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=F16)                      # noqa: E731
+    kp, vp, emb, wq, wk, wv, out_w = rnd(Hkv, P, D), rnd(Hkv, P, D), rnd(V, 64), rnd(64, H * D) / 8, rnd(64, Hkv * D) / 8, rnd(64, Hkv * D) / 8, rnd(H * D, V) / 22
+    question = torch.randint(0, V, (B, T), generator=g, device="cuda")
+
+    def begin():
+        s = dict(k=torch.full((B, Hkv, rows, D), float("nan"), dtype=F16, device="cuda"), n=dev_lens([0]), tok=torch.zeros(B, 1, dtype=torch.int64, device="cuda"),
+                 hist=torch.zeros(B, rows, dtype=torch.int64, device="cuda"), nt=dev_lens([T] * B), np=dev_lens([T] * B),
+                 scratch=ops.new_greedy_scratch(kp.device, B), rep=torch.full((1,), 1.3, device="cuda"), freq=torch.full((1,), 0.5, device="cuda"))
+        s["v"] = s["k"].clone()
+        s["hist"][:, :T] = question
+        x = emb[question]
+        heads = lambda w, h: (x @ w).view(B, T, h, D).transpose(1, 2)                            # noqa: E731
+        s["k"][:, :, :T], s["v"][:, :, :T] = heads(wk, Hkv), heads(wv, Hkv)
+        a = ops.decode_shared_prefix_attention(heads(wq, H), kp, vp, s["k"], s["v"], s["n"], D ** -0.5)
+        choose(s, a[:, -1:])
+        return s
+
+    def choose(s, a):
+        logits = (a @ out_w).view(B, V)
+        x = ops.decode_penalties(logits, s["hist"], s["nt"], s["np"], repetition=s["rep"], frequency=s["freq"])
+        ops.decode_greedy(x[:, None], s["scratch"], s["tok"])
+        s["hist"].scatter_(1, s["nt"].long()[:, None], s["tok"])
+        s["nt"].add_(1)
+
+    def step(s):
+        x = emb[s["tok"][:, 0]][:, None]
+        heads = lambda w, h: (x @ w).view(B, 1, h, D).transpose(1, 2)                            # noqa: E731
+        ops.decode_append(s["k"], s["v"], heads(wk, Hkv), heads(wv, Hkv), s["n"])
+        choose(s, ops.decode_shared_prefix_attention(heads(wq, H), kp, vp, s["k"], s["v"], s["n"], D ** -0.5))
+
+    eager = begin()
+    for _ in range(steps):
+        step(eager)
+    s = begin()
+    step(s)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(s)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(steps - 1):
+        graph.replay()
+        torch.cuda.synchronize()
+        eager["k"].nan_to_num().sum()                                # the program's own work between the replays
+    assert int(s["n"]) == int(eager["n"]) == T + steps
+    assert torch.equal(s["hist"], eager["hist"]) and torch.equal(s["nt"], eager["nt"])
+    assert len(set(s["hist"][0, T:T + steps + 1].tolist())) > 1
