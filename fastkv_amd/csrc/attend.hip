@@ -177,7 +177,7 @@ struct AttState { float m, l; };
 
 // 16 bytes per active lane from memory to shared memory: lane l's land at lds + OFF + 16 l.  Written as assembly because the compiler, which
 // cannot tell the tile in flight from the one being read, waits for every such load in front of the next transposing read; the waits are
-// att_landed's, and nothing of these loads is in a register.
+// att_landed's, and nothing of these loads is in a register.  m0 is reserved: the compiler sets it where it needs it and keeps nothing in it.
 template <int OFF> __device__ __forceinline__ void att_bring(att_u4 buffer, int offset, int base_offset, uint32_t lds)
 {
     asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
@@ -734,7 +734,9 @@ struct AttPlan { int rwp, rw, packed_tiles, packed_split, tiles, split, slots; i
 // Into how many slices the keys of `items` items (n keys each, `per` keys a step of the workgroup) are cut: the least of a plain sum of times in
 // us, whose constants are measured -- what a workgroup takes for itself (2.5) and per step (rows: 1.55 for 128 x 64 at 128 dims alone on its
 // compute unit, 2.0 each for two; keys: 1.0, and what the memory gives), and the join (3.5, and the slices' fp32 sums written and read).
-static int att_cut(int64_t items, int64_t n, int per, double step, double step2, int64_t rows, int D, int extra)
+// `beside`: the time of other items that run meanwhile; `took`, where given, gets that of these.
+static int att_cut(int64_t items, int64_t n, int per, double step, double step2, int64_t rows, int D, int extra, double beside = 0.0,
+                   double *took = nullptr)
 {
     const int64_t steps = (n + per - 1) / per;
     int best = 1;
@@ -744,8 +746,14 @@ static int att_cut(int64_t items, int64_t n, int per, double step, double step2,
         const int64_t wgs = items * s, each = (steps + s - 1) / s;
         const int64_t full = wgs / 512, rest = wgs % 512;
         double t = (double)(full * (2.5 + each * step2)) + (rest ? 2.5 + each * (rest > 256 ? step2 : step) : 0.0);
+        const double alone = t;
+        if (t < beside) t = beside;
         if (s + extra > 1) t += 3.5 + rows * (s + extra) * (D + 2) * 8.0 / 4e6;
-        if (t < least * 0.99) { least = t; best = s; }
+        if (t < least * 0.99) {
+            least = t;
+            best = s;
+            if (took) *took = alone;
+        }
     }
     return best;
 }
@@ -761,12 +769,18 @@ static AttPlan att_plan(int B, int H, int Hkv, int D, int T, int64_t keys, int64
         P.rwp = R <= few ? 1 : 4;
         P.rw = TG <= few ? 1 : 4;
         P.packed_tiles = (int)((R + 32 * P.rwp - 1) / (32 * P.rwp));
-        P.packed_split = P.rwp == 1 ? att_cut((int64_t)Hkv * P.packed_tiles, prefix, 128, kstep, 2 * kstep, all, D, 1)
-                                    : att_cut((int64_t)Hkv * P.packed_tiles, prefix, 64, step, step2, all, D, 1);
+        // The requests' own rows run beside the prefix: they are cut where they are long (4 requests of 8192 rows, 32 heads on 8, behind 512 shared
+        // ones: 77 us in one piece each, 31 so; 2 of 16384, 16 heads on 2: 107 and 17), not where they take little longer
+        // than the prefix does (8 of 512, 4 tokens each, behind 4096: 22.5 us whole, 24.0 cut).
+        double prefix_takes = 0.0;
+        P.packed_split = P.rwp == 1 ? att_cut((int64_t)Hkv * P.packed_tiles, prefix, 128, kstep, 2 * kstep, all, D, 1, 0.0, &prefix_takes)
+                                    : att_cut((int64_t)Hkv * P.packed_tiles, prefix, 64, step, step2, all, D, 1, 0.0, &prefix_takes);
         P.tiles = (int)((TG + 32 * P.rw - 1) / (32 * P.rw));
-        P.split = 1;
-        P.slots = P.packed_split + 1;
-        P.blocks = (int64_t)Hkv * P.packed_tiles * P.packed_split + (int64_t)B * Hkv * P.tiles;
+        const double beside = prefix_takes * 1.25;
+        P.split = P.rw == 1 ? att_cut((int64_t)B * Hkv * P.tiles, keys, 128, kstep, 2 * kstep, all, D, P.packed_split, beside)
+                            : att_cut((int64_t)B * Hkv * P.tiles, keys, 64, step, step2, all, D, P.packed_split, beside);
+        P.slots = P.packed_split + P.split;
+        P.blocks = (int64_t)Hkv * P.packed_tiles * P.packed_split + (int64_t)B * Hkv * P.tiles * P.split;
         return P;
     }
     P.rwp = P.rw = TG <= few ? 1 : 4;

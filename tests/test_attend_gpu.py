@@ -157,6 +157,8 @@ PREFIX = [
     (3, 4, 2, 128, 1, 100, 16, F16, [-1, 5, 15]),             # an idle request
     (2, 4, 1, 128, 6, 90, 64, BF16, [-3, 30]),                # left padding
     (2, 4, 1, 64, 40, 90, 64, F16, [-20, 24]),
+    (2, 8, 2, 128, 1, 150, 3500, F16, [3490, 100]),           # own rows far longer than the prefix: cut as well
+    (2, 8, 2, 64, 5, 40, 1900, BF16, [1800, 3]),
 ]
 
 
