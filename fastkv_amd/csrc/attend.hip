@@ -27,8 +27,8 @@
 // Work too small to fill the chip is cut along the keys; slices leave {m, l, O} in a workspace and attend_join adds them up.
 //
 // What bounds it, measured (H 32, Hkv 8, D 128):
-//   prompts   the matrix pipe, the vector pipe and the clock together: 8k tokens, window 4096: 0.44 ms, 940 TFLOP/s (an 8192^3 library product:
-//             1110); 32k: 2.18 ms, 950.  Per tile of a wave 1024 cycles of products beside ~1000 of vector work; the clock falls to
+//   prompts   the matrix pipe, the vector pipe and the clock together: 8k tokens, window 4096: 0.43 ms, 960 TFLOP/s (an 8192^3 library product:
+//             1110); 32k: 2.12 ms, 970.  Per tile of a wave 1024 cycles of products beside ~1000 of vector work; the clock falls to
 //             1.95 GHz under it.  Leaving out the exponentials / the loads / the second product gives 7 / 14 / 12 %: nothing alone bounds it.
 //             Slower: two groups of waves held half a tile apart by barriers (0.53 ms), raised wave priorities (+3 %), exponentials
 //             interleaved with products by hand (+3 %), 32-key tiles (registers spill at three waves per SIMD).
@@ -294,19 +294,37 @@ template <int D, bool BF, int NB> __device__ __forceinline__ void att_scores(con
         for (int kb = 0; kb < NB; ++kb) S[kb] = att_mfma<BF>(*reinterpret_cast<const att_u4 *>(at[s % NX] + s / NX * NX * 16 + kb * 32 * D), Q[s], S[kb]);
 }
 
-// the running softmax over a tile's scores, u0 its first key; `edge`: some row may not see some key.  P^T comes out as the second operand of V^T P^T.
+// keys u0 .. of a tile that this lane's row (position p) does not see
+template <int NB> __device__ __forceinline__ void att_mask(att_f16 (&S)[NB], const AttKeys &K, int u0, int p)
+{
+    const AttSees sees(K, u0 + 4 * (threadIdx.x >> 5 & 1), p);
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[kb][r] = sees(kb * 32 + (r & 3) + 8 * (r >> 2)) ? S[kb][r] : -INFINITY;
+}
+// a tile's weights 2^(c (s - m)): P^T as the second operand of V^T P^T, and their sum
+template <bool BF, int NB> __device__ __forceinline__ float att_weights(const att_f16 (&S)[NB], att_u4 (&P)[NB * 2], float m, float c)
+{
+    const float mc = (m == -INFINITY ? 0.0f : m * c) - (BF ? 0.0f : ATT_LIFT);
+    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][r], c, -mc)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][r + 1], c, -mc));
+            l0 += a;
+            l1 += b;
+            P[kb * 2 + (r >> 3)][(r & 7) >> 1] = att_pack<BF>(a, b);
+        }
+    return l0 + l1;
+}
+// the running softmax over a tile's scores, u0 its first key; `edge`: some row may not see some key
 template <int D, bool BF, int NB>
 __device__ __forceinline__ void att_softmax(att_f16 (&S)[NB], att_u4 (&P)[NB * 2], att_f16 (&O)[D / 32], AttState &st, float c, const AttKeys &K, int u0,
                                             int p, bool edge)
 {
-    const int hi = threadIdx.x >> 5 & 1;
-    if (edge) {
-        const AttSees sees(K, u0 + 4 * hi, p);
-#pragma unroll
-        for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) S[kb][r] = sees(kb * 32 + (r & 3) + 8 * (r >> 2)) ? S[kb][r] : -INFINITY;
-    }
+    if (edge) att_mask<NB>(S, K, u0, p);
     float tm = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
@@ -323,18 +341,7 @@ __device__ __forceinline__ void att_softmax(att_f16 (&S)[NB], att_u4 (&P)[NB * 2
 #pragma unroll
             for (int r = 0; r < 16; ++r) O[db][r] *= f;
     }
-    const float mc = (st.m == -INFINITY ? 0.0f : st.m * c) - (BF ? 0.0f : ATT_LIFT);
-    float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-    for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][r], c, -mc)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][r + 1], c, -mc));
-            l0 += a;
-            l1 += b;
-            P[kb * 2 + (r >> 3)][(r & 7) >> 1] = att_pack<BF>(a, b);
-        }
-    st.l += l0 + l1;
+    st.l += att_weights<BF, NB>(S, P, st.m, c);
 }
 
 // O^T += V^T P^T
@@ -394,6 +401,42 @@ __device__ __forceinline__ void att_wild_rows(const att_u4 (&P)[NB * 2], att_f16
     }
 }
 
+// Those pieces, behind the loop over the tiles and only where one was taken out: the partly seen tiles once more, their weights from the final
+// maximum.  In the loop its registers cost every call (8k tokens, window 4096: 256 dims 1.49 ms instead of 1.36, where O moved between the
+// register files in every tile; 128 dims 0.444 instead of 0.429).
+// NW = 4: the workgroup's tiles, 1: a wave's own.
+template <int D, bool BF, int NB, int NW>
+__device__ __forceinline__ void att_wild_tiles(const att_u4 (&Q)[D / 16], att_f16 (&O)[D / 32], const AttState &st, float c, const AttKeys &K, int u, int step,
+                                               int p, uint16_t *ks, int w, unsigned long long *word)
+{
+    typedef AttLoad<D, NB, NW> Load;
+    uint16_t *vs = ks + 32 * NB * D;
+#pragma unroll 1
+    for (; u < K.N; u += step) {
+        if (K.lean(u)) continue;
+        att_read_done();
+        if (NW > 1) __syncthreads();
+        if ((NW > 1 ? threadIdx.x : threadIdx.x & 63) == 0) *word = 0;
+        Load::template issue<false>(K, u, ks, w);
+        Load::template issue<true>(K, u, vs, w);
+        att_landed<0>();
+        if (NW > 1) __syncthreads();
+        asm volatile("" ::: "memory");
+        Load::template scan<BF>(vs, w, word);
+        asm volatile("" ::: "memory");                       // (one wave's accesses to shared memory are in order)
+        if (NW > 1) __syncthreads();
+        const unsigned long long x = *word;
+        const uint64_t wild = (uint64_t)att_uniform((uint32_t)(x >> 32)) << 32 | att_uniform((uint32_t)x);
+        if (!wild) continue;
+        att_f16 S[NB];
+        att_u4 P[NB * 2];
+        att_scores<D, BF, NB>(ks, Q, S);
+        att_mask<NB>(S, K, u, p);
+        att_weights<BF, NB>(S, P, st.m, c);
+        att_wild_rows<D, BF, NB>(P, O, K, u, p, wild);
+    }
+}
+
 __device__ __forceinline__ int att_len(const AttendArgs &A, int b)
 {
     const int n = A.len ? A.len[(int64_t)b * A.len_step] : A.len_all;
@@ -445,7 +488,7 @@ template <int D, bool BF, int RW, bool SAME> __device__ __forceinline__ void att
 {
     constexpr int NB = RW == 4 ? 2 : 1, KT = 32 * NB, KW = 4 / RW;
     constexpr int TILE = KT * D;                             // elements of a K (or V) tile
-    __shared__ unsigned long long s_wild[4];                // (rows: three in turn)
+    __shared__ unsigned long long s_wild[4];                // keys whose V rows had a piece taken out: not 0 if any (keys: per wave)
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hi = lane >> 5;
     const int TG = A.T * A.G, R = it.packed ? A.B * TG : TG;
     // ---- this lane's query row
@@ -510,7 +553,7 @@ template <int D, bool BF, int RW, bool SAME> __device__ __forceinline__ void att
     if (RW == 4) {
         typedef AttLoad<D, NB, 4> Load;
         const bool idle = wrow0 >= R;
-        if (tid < 3) s_wild[tid] = 0;
+        if (tid == 0) s_wild[0] = 0;
         if (u_lo < K.N) {
             Load::template issue<false>(K, u_lo, smem, w);
             Load::template issue<true>(K, u_lo, smem + TILE, w);
@@ -520,11 +563,11 @@ template <int D, bool BF, int RW, bool SAME> __device__ __forceinline__ void att
         bool lean = K.lean(u_lo);
         if (!SAME && u_lo < K.N && !lean) Load::template scan<BF>(smem + TILE, w, &s_wild[0]);
         __syncthreads();
-        int at = 0, wl = 0;                                   // the tile's place in shared memory, its word of s_wild
+        int at = 0;                                           // the tile's place in shared memory
         for (int u = u_lo; u < K.N; u += KT) {
             const uint16_t *cur = smem + at;
             uint16_t *nxt = smem + (at ^ 2 * TILE);
-            const int un = u + KT, wn = wl == 2 ? 0 : wl + 1;
+            const int un = u + KT;
             const bool more = un < K.N, next_lean = K.lean(un);
             if (more) {                                       // (the other buffer was last read before the barrier)
                 Load::template issue<false>(K, un, nxt, w);
@@ -539,20 +582,19 @@ template <int D, bool BF, int RW, bool SAME> __device__ __forceinline__ void att
                 att_scores<D, BF, NB>(cur, Q, S);
                 att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, !lean);
                 att_values<D, BF, NB>(cur + TILE, P, O);
-                if (!SAME && !lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, s_wild[wl]);
             }
             att_landed<0>();
-            if (!SAME && more && !next_lean) Load::template scan<BF>(nxt + TILE, w, &s_wild[wn]);      // (a lane looks at what it brought itself)
-            if (!SAME && tid == 0) s_wild[wn == 2 ? 0 : wn + 1] = 0;     // last read a tile ago, written a tile from now
+            if (!SAME && more && !next_lean) Load::template scan<BF>(nxt + TILE, w, &s_wild[0]);      // (a lane looks at what it brought itself)
             __syncthreads();
             at ^= 2 * TILE;
-            wl = wn;
             lean = next_lean;
         }
+        if (!SAME && s_wild[0]) att_wild_tiles<D, BF, NB, 4>(Q, O, st, A.c, K, u_lo, KT, p, smem, w, &s_wild[0]);
     } else {
         typedef AttLoad<D, NB, 1> Load;
         uint16_t *ks = smem + w * 2 * TILE, *vs = ks + TILE;
         int u = u_lo + w * KT;
+        if (!SAME && lane == 0) s_wild[w] = 0;
         bool whole = K.whole(u);
         if (u < K.N) {
             Load::template issue<false>(K, u, ks, 0);
@@ -569,21 +611,17 @@ template <int D, bool BF, int RW, bool SAME> __device__ __forceinline__ void att
             att_softmax<D, BF, NB>(S, P, O, st, A.c, K, u, p, !lean);
             if (next_whole) att_landed<Load::CH>();
             else att_landed<0>();
-            uint64_t wild = 0;
             if (!SAME && !lean) {
-                if (lane == 0) s_wild[w] = 0;
-                asm volatile("" ::: "memory");
                 Load::template scan<BF>(vs, 0, &s_wild[w]);  // (one wave's accesses to shared memory are in order)
                 asm volatile("" ::: "memory");
-                wild = s_wild[w];
             }
             att_values<D, BF, NB>(vs, P, O);
-            if (!SAME && !lean) att_wild_rows<D, BF, NB>(P, O, K, u, p, wild);
             att_read_done();
             if (more) Load::template issue<true>(K, un, vs, 0);
             u = un;
             whole = next_whole;
         }
+        if (!SAME && s_wild[w]) att_wild_tiles<D, BF, NB, 1>(Q, O, st, A.c, K, u_lo + w * KT, KT * KW, p, ks, 0, &s_wild[w]);
     }
     st.l = att_other_half_sum(st.l);
 

@@ -89,6 +89,27 @@ def test_rows_that_nothing_sees_may_hold_anything(D, dtype, T):
     check(got, ref, bound)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, F16), (256, BF16)])
+@pytest.mark.parametrize("T", [9, 300])
+def test_infinities_in_many_tiles(D, dtype, T):
+    """Infinities and NaN in V rows of several partly seen tiles, in front of them and behind them, while the running maximum moves: the other
+    dims of their pieces keep their values, and rows that do not see them stay finite."""
+    from fastkv_amd import ops
+    H, Hkv, n, window = 4, 2, 700, 260
+    rows = n + T
+    q, k, v = make(D + T, 1, H, Hkv, D, T, rows, dtype)
+    k *= torch.linspace(0.2, 2.5, rows).to(dtype)[None, None, :, None]
+    for i, j in enumerate(range(n - window - 3, rows, 37)):
+        v[0, i % Hkv, j, (i * 11) % D] = [float("inf"), -float("inf"), float("nan")][i % 3]
+    v[0, 0, 2, 3] = float("inf")                               # a sink
+    v[0, 1, rows - 1] = float("nan")                           # a whole row, the last query's alone
+    for sinks in (0, 4):
+        got = ops.window_attention(q.cuda(), k.cuda(), v.cuda(), window=window, sinks=sinks)
+        ref, bound = attend(q, window_rows(k.double(), v.double(), [n], T, window, sinks, Hkv, H), D ** -0.5)
+        assert torch.isfinite(ref).any() and not torch.isfinite(ref).all()
+        check(got, ref, bound)
+
+
 def test_one_strong_key_among_many_weak_ones():
     """Thousands of keys 2^-15 of the strongest: each p is small for 16 bits, together they weigh as much as the strong one."""
     from fastkv_amd import ops
