@@ -800,10 +800,12 @@ static AttPlan att_plan(int B, int H, int Hkv, int D, int T, int64_t keys, int64
 {
     AttPlan P = {};
     const int64_t TG = (int64_t)T * (H / Hkv), all = (int64_t)B * H * T;
-    const int few = T == 1 || D < 256 ? 32 : 0;               // rows up to which the keys shape is taken
     const double step = D * 1.55 / 128, step2 = D * 2.0 / 128, kstep = D * 1.0 / 128;
     if (prefix > 0 && TG < 128 && B > 1) {                    // rows of all requests in one tile: the prefix is read once, not once per request
         const int64_t R = B * TG;
+        // rows up to which the keys shape is taken.  Several tokens of 256 dims: 8 requests of 2 / 8 tokens behind 6553 rows 36.7 / 53 us without
+        // it, 39.9 / 57 with it; not so where there is a window alone (2 requests of 2 / 8 tokens, window 4096: 35 / 38 us without, 26 / 28 with).
+        const int few = T == 1 || D < 256 ? 32 : 0;
         P.rwp = R <= few ? 1 : 4;
         P.rw = TG <= few ? 1 : 4;
         P.packed_tiles = (int)((R + 32 * P.rwp - 1) / (32 * P.rwp));
@@ -821,7 +823,7 @@ static AttPlan att_plan(int B, int H, int Hkv, int D, int T, int64_t keys, int64
         P.blocks = (int64_t)Hkv * P.packed_tiles * P.packed_split + (int64_t)B * Hkv * P.tiles * P.split;
         return P;
     }
-    P.rwp = P.rw = TG <= few ? 1 : 4;
+    P.rwp = P.rw = TG <= 32 ? 1 : 4;
     const int per = 32 * P.rw;
     P.tiles = (int)((TG + per - 1) / per);
     const int64_t items = (int64_t)B * Hkv * P.tiles;
@@ -850,9 +852,9 @@ static int att_launch(AttendArgs &A, const AttPlan &P, int advance, int32_t *len
     {
         ProfScope ps_(K_ATTEND, st);
         const dim3 grid((unsigned)P.blocks), block(ATT_THREADS);
-        constexpr bool SEVERAL = D == 256;                    // (no keys shape for several tokens of 256 dims: att_plan)
+        constexpr bool SEVERAL = D == 256;                    // (several tokens of 256 dims never have the two shapes side by side: att_plan)
         if (P.rwp == 1 && A.T == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 1, 1, true>), grid, block, 0, st, A);
-        else if (P.rwp == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 1, 1, SEVERAL>), grid, block, 0, st, A);
+        else if (P.rwp == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 1, 1, false>), grid, block, 0, st, A);
         else if (P.rw == 1 && A.T == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 4, 1, true>), grid, block, 0, st, A);
         else if (P.rw == 1) hipLaunchKernelGGL((attend_kernel<D, BF, 4, 1, SEVERAL>), grid, block, 0, st, A);
         else hipLaunchKernelGGL((attend_kernel<D, BF, 4, 4, false>), grid, block, 0, st, A);
