@@ -777,13 +777,16 @@ static int att_cut(int64_t items, int64_t n, int per, double step, double step2,
                    double *took = nullptr)
 {
     const int64_t steps = (n + per - 1) / per;
+    // 256 dims: one workgroup per compute unit, 3.5 us a step (cut as if there were two: 2 x 512 tokens, window 4096 232 us, 207 so; 64 requests
+    // behind 32768 rows 188, 167)
+    const int at_once = D > 128 ? 256 : 512;
     int best = 1;
     double least = 1e30;
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
         if (s > steps) break;
         const int64_t wgs = items * s, each = (steps + s - 1) / s;
-        const int64_t full = wgs / 512, rest = wgs % 512;
-        double t = (double)(full * (2.5 + each * step2)) + (rest ? 2.5 + each * (rest > 256 ? step2 : step) : 0.0);
+        const int64_t full = wgs / at_once, rest = wgs % at_once;
+        double t = (double)(full * (2.5 + each * (D > 128 ? step : step2))) + (rest ? 2.5 + each * (rest > 256 ? step2 : step) : 0.0);
         const double alone = t;
         if (t < beside) t = beside;
         if (s + extra > 1) t += 3.5 + rows * (s + extra) * (D + 2) * 8.0 / 4e6;
@@ -809,7 +812,7 @@ static AttPlan att_plan(int B, int H, int Hkv, int D, int T, int rows, int64_t s
 {
     AttPlan P = {};
     const int64_t TG = (int64_t)T * (H / Hkv), all = (int64_t)B * H * T;
-    const double step = D * 1.55 / 128, step2 = D * 2.0 / 128, kstep = D * 1.0 / 128;
+    const double step = D > 128 ? 3.5 : D * 1.55 / 128, step2 = D * 2.0 / 128, kstep = D * 1.0 / 128;
     if (prefix > 0 && TG < 128 && B > 1) {                    // rows of all requests in one tile: the prefix is read once, not once per request
         const int64_t R = B * TG;
         // rows up to which the keys shape is taken.  Several tokens of 256 dims: 8 requests of 2 / 8 tokens behind 6553 rows 36.7 / 53 us without
