@@ -38,7 +38,7 @@ class SPWindow(ctypes.Structure):
 EXPORTS = ["fastkv_workspace_bytes", "fastkv_workspace_init", "fastkv_update_kv_f16", "fastkv_update_kv_strided_f16", "fastkv_score_f16", "fastkv_select_f16",
            "fastkv_select_workspace_bytes", "fastkv_compact_f16", "fastkv_compact_ranked_f16", "fastkv_gather_rows", "fastkv_tsp_propagate", "fastkv_head_sum_f16", "fastkv_sp_workspace_bytes", "fastkv_sp_logits_f16", "fastkv_sp_rowmax_f16", "fastkv_sp_rowsum_f16",
            "fastkv_sp_scores_f16", "fastkv_sp_pack_f16", "fastkv_sp_unpack_f16", "fastkv_sp_pick",
-           "fastkv_sp_compact_f16", "fastkv_decode_workspace_bytes", "fastkv_decode_append_f16", "fastkv_decode_attention_f16",
+           "fastkv_sp_compact_f16", "fastkv_decode_workspace_bytes", "fastkv_decode_append_f16", "fastkv_decode_append", "fastkv_decode_attention_f16",
            "fastkv_decode_rmsnorm_f16", "fastkv_decode_rope_f16", "fastkv_decode_silu_mul_f16", "fastkv_decode_greedy_f16", "fastkv_decode_rotary_f16", "fastkv_decode_gemv_f16", "fastkv_update_kv_ptrs_f16", "fastkv_fused_entries_f16", "fastkv_pool_f16", "fastkv_decode_step_attention_f16", "fastkv_attend_workspace_bytes", "fastkv_window_attention", "fastkv_shared_prefix_attention", "fastkv_decode_penalties", "fastkv_debug_contract", "fastkv_debug_mfma16", "fastkv_debug_granule_areas", "fastkv_debug_occupy", "fastkv_debug_fused_placement", "fastkv_placement_violations", "fastkv_set_placement_policy", "fastkv_set_no_wait_mode", "fastkv_set_fused_rolling", "fastkv_no_wait_mode", "fastkv_last_status", "fastkv_profile_enable",
            "fastkv_profile_kernels", "fastkv_profile_kernel_name", "fastkv_profile_read", "fastkv_strerror", "fastkv_version"]
 
@@ -106,6 +106,8 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
     L.fastkv_decode_workspace_bytes.restype = sz
     L.fastkv_decode_append_f16.argtypes = [ci, ci, ci, vp, i64p, vp, i64p, vp, vp, i64p, ci, vp, vp]
     L.fastkv_decode_append_f16.restype = ci
+    L.fastkv_decode_append.argtypes = [ci, ci, ci, vp, i64p, vp, i64p, vp, vp, i64p, ci, vp, ci, vp]
+    L.fastkv_decode_append.restype = ci
     L.fastkv_decode_attention_f16.argtypes = [ci, ci, ci, ci, vp, i64p, vp, vp, i64p, ci, vp, ctypes.c_float, ci, vp, vp, sz, vp]
     L.fastkv_decode_attention_f16.restype = ci
     L.fastkv_decode_rmsnorm_f16.argtypes = [vp, i64, i64, ci, vp, ctypes.c_float, vp, vp]

@@ -3,7 +3,7 @@
 // /root/reference/benchmark/e2e.py:72-93 times it).  Here the cache is a pre-sized slab [B,Hkv,rows,D] per layer
 // (fastkv_amd/cache.py) whose current length lives in DEVICE memory, so the whole decode step has static shapes and can be
 // replayed from a HIP graph:
-//   decode_append    the step's K/V row -> slab row `len`                        (one 16-B piece per thread)
+//   decode_append    the step's K/V row -> slab row `len`, one length for the batch or one per request (one 16-B piece per thread)
 //   decode_partial   GQA attention of the G query heads of a KV head over a slice of the len+1 rows: scores with one cache
 //                    row per lane (the row's 2*D bytes in 16-B loads), online softmax per wave, P.V with the lanes across
 //                    head_dim (coalesced 4-B loads of V rows, probabilities from LDS) -> {max, sum, o[D]} per slice
@@ -25,11 +25,12 @@ template <int LPR>
 __global__ void __launch_bounds__(64) decode_append_kernel(const uint16_t *__restrict__ k_new, int64_t kn_b, int64_t kn_h,
                                                           const uint16_t *__restrict__ v_new, int64_t vn_b, int64_t vn_h,
                                                           uint16_t *__restrict__ kslab, uint16_t *__restrict__ vslab, int64_t s_b,
-                                                          int64_t s_h, int64_t s_r, int rows, const int32_t *__restrict__ len_dev)
+                                                          int64_t s_h, int64_t s_r, int rows, const int32_t *__restrict__ len_dev,
+                                                          int len_step)
 {
     const int h = blockIdx.x, b = blockIdx.y, sub = threadIdx.x;
-    int len = *len_dev;
-    if (sub >= LPR) return;
+    int len = len_dev[(int64_t)b * len_step];
+    if (sub >= LPR || len < 0) return;                           // an idle request has no row: nothing is stored in front of the slab
     if (len >= rows) len = rows - 1;                             // a full slab overwrites its last row instead of its neighbour (the host sizes it)
     const uint4 kv = *reinterpret_cast<const uint4 *>(k_new + b * kn_b + h * kn_h + sub * 8);
     const uint4 vv = *reinterpret_cast<const uint4 *>(v_new + b * vn_b + h * vn_h + sub * 8);
@@ -350,12 +351,13 @@ using namespace fk;
 
 extern "C" {
 
-int fastkv_decode_append_f16(int32_t B, int32_t Hkv, int32_t D, const void *k_new, const int64_t kn_strides[2], const void *v_new,
-                             const int64_t vn_strides[2], void *kslab, void *vslab, const int64_t slab_strides[3], int32_t rows,
-                             const int32_t *len_dev, void *stream)
+int fastkv_decode_append(int32_t B, int32_t Hkv, int32_t D, const void *k_new, const int64_t kn_strides[2], const void *v_new,
+                         const int64_t vn_strides[2], void *kslab, void *vslab, const int64_t slab_strides[3], int32_t rows,
+                         const int32_t *len_dev, int32_t len_step, void *stream)
 {
     if (B < 1 || Hkv < 1 || rows < 1 || !k_new || !v_new || !kslab || !vslab || !len_dev || !kn_strides || !vn_strides || !slab_strides)
         return FASTKV_EINVAL;
+    if (len_step < 0 || len_step > 1) return FASTKV_EINVAL;
     if (D != 64 && D != 128 && D != 256) return FASTKV_EUNSUPPORTED;
     if (((uintptr_t)k_new | (uintptr_t)v_new | (uintptr_t)kslab | (uintptr_t)vslab) & 15) return FASTKV_EINVAL;
     for (int i = 0; i < 2; ++i) if ((kn_strides[i] & 7) || (vn_strides[i] & 7)) return FASTKV_EINVAL;
@@ -366,12 +368,19 @@ int fastkv_decode_append_f16(int32_t B, int32_t Hkv, int32_t D, const void *k_ne
 #define FK_APP(LPRV)                                                                                                                \
     hipLaunchKernelGGL((decode_append_kernel<LPRV>), grid, dim3(64), 0, st, (const uint16_t *)k_new, kn_strides[0], kn_strides[1],  \
                        (const uint16_t *)v_new, vn_strides[0], vn_strides[1], (uint16_t *)kslab, (uint16_t *)vslab, slab_strides[0], \
-                       slab_strides[1], slab_strides[2], rows, len_dev)
+                       slab_strides[1], slab_strides[2], rows, len_dev, len_step)
     if (D == 64) FK_APP(8);
     else if (D == 128) FK_APP(16);
     else FK_APP(32);
 #undef FK_APP
     return hipGetLastError() == hipSuccess ? FASTKV_OK : FASTKV_ELAUNCH;
+}
+
+int fastkv_decode_append_f16(int32_t B, int32_t Hkv, int32_t D, const void *k_new, const int64_t kn_strides[2], const void *v_new,
+                             const int64_t vn_strides[2], void *kslab, void *vslab, const int64_t slab_strides[3], int32_t rows,
+                             const int32_t *len_dev, void *stream)
+{
+    return fastkv_decode_append(B, Hkv, D, k_new, kn_strides, v_new, vn_strides, kslab, vslab, slab_strides, rows, len_dev, 0, stream);
 }
 
 int fastkv_decode_attention_f16(int32_t B, int32_t H, int32_t Hkv, int32_t D, const void *q, const int64_t q_strides[2],

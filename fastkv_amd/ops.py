@@ -324,22 +324,38 @@ DECODE_NSPLIT = int(os.environ.get("FASTKV_DECODE_NSPLIT", "16"))
 
 
 def decode_append(kslab: torch.Tensor, vslab: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, len_dev: torch.Tensor) -> None:
-    """Slab row `len_dev[0]` <- the step's K/V row ([B,Hkv,1,D]); the length itself is advanced by decode_attention."""
-    _require_cuda(kslab, vslab, k_new, v_new, len_dev)
+    """Slab row `len_dev[b]` of request b <- the step's K/V row ([B,Hkv,1,D], fp16 or bf16 as the slabs); `len_dev` int32 [1] (one length
+    for the batch) or [B].  A negative length is an idle request: nothing is stored; a full slab's last row is overwritten.  The length
+    itself is advanced by the attention behind it: decode_attention (one length), decode_window_attention or
+    decode_shared_prefix_attention (one or [B])."""
     B, Hkv, rows, D = kslab.shape
+    if kslab.dtype not in _ATTEND_DTYPE or any(t.dtype is not kslab.dtype for t in (vslab, k_new, v_new)):
+        raise TypeError(f"fastkv_amd.decode_append: slabs and rows of one type, fp16 or bf16, expected; got "
+                        f"{[t.dtype for t in (kslab, vslab, k_new, v_new)]}")
+    if len_dev.dtype is not torch.int32 or not (len_dev.numel() == 1 or (len_dev.shape == (B,) and len_dev.is_contiguous())):
+        raise ValueError(f"fastkv_amd.decode_append: len_dev must be a contiguous int32 tensor of 1 or {B} lengths")
+    _require_cuda(kslab, vslab, k_new, v_new, len_dev)
+    assert vslab.shape == kslab.shape
     assert k_new.shape == (B, Hkv, 1, D) and v_new.shape == k_new.shape and k_new.stride(3) == 1 and v_new.stride(3) == 1
-    assert kslab.stride() == vslab.stride() and kslab.stride(3) == 1 and len_dev.dtype == torch.int32
+    assert kslab.stride() == vslab.stride() and kslab.stride(3) == 1
     I2, I3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
-    rc = load().fastkv_decode_append_f16(B, Hkv, D, k_new.data_ptr(), I2(k_new.stride(0), k_new.stride(1)), v_new.data_ptr(),
-                                         I2(v_new.stride(0), v_new.stride(1)), kslab.data_ptr(), vslab.data_ptr(),
-                                         I3(*kslab.stride()[:3]), rows, len_dev.data_ptr(), _stream())
-    check(rc, "decode_append")
+    _launch("decode_append", kslab.get_device(), load().fastkv_decode_append, B, Hkv, D, k_new.data_ptr(), I2(k_new.stride(0), k_new.stride(1)),
+            v_new.data_ptr(), I2(v_new.stride(0), v_new.stride(1)), kslab.data_ptr(), vslab.data_ptr(), I3(*kslab.stride()[:3]), rows,
+            len_dev.data_ptr(), 1 if len_dev.numel() > 1 else 0)
+
+
+def _one_length(what: str, len_dev: torch.Tensor) -> None:
+    # (the dense decode kernels read and advance len_dev[0] alone: requests of other lengths would be answered from the first one's rows)
+    if len_dev.dtype is not torch.int32 or len_dev.numel() != 1:
+        raise ValueError(f"fastkv_amd.{what}: one int32 length for the batch expected, got {len_dev.dtype} {tuple(len_dev.shape)} (one per "
+                         "request: decode_window_attention)")
 
 
 def decode_attention(q: torch.Tensor, kslab: torch.Tensor, vslab: torch.Tensor, len_dev: torch.Tensor, scaling: float,
                      nsplit: int = 0, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """GQA attention of q [B,H,1,D] over slab rows 0 .. len_dev[0] (inclusive: the row decode_append just wrote) -> fp16
     [B,1,H*D]; advances len_dev on the device.  Static shapes: capturable in a HIP graph."""
+    _one_length("decode_attention", len_dev)
     _require_cuda(q, kslab, vslab, len_dev)
     B, H, one, D = q.shape
     Hkv, rows = kslab.shape[1], kslab.shape[2]
@@ -570,7 +586,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 def decode_window_attention(q: torch.Tensor, kslab: torch.Tensor, vslab: torch.Tensor, len_dev: torch.Tensor, scaling: float,
                             window: Optional[int] = None, sinks: int = 0, advance: bool = True) -> torch.Tensor:
     """`decode_attention` for a model with a sliding window: q [B,H,1,D] over the slab rows that `window` and `sinks` leave of rows
-    0 .. len_dev (inclusive: the row decode_append just wrote) -> [B,1,H*D]; len_dev (int32 [1] or [B]) moves on by one on the device
+    0 .. len_dev (inclusive: the row decode_append just wrote, with the same lengths) -> [B,1,H*D]; len_dev (int32 [1] or [B]) moves on by one on the device
     unless `advance` is False.  A negative length is an idle request: zeros, and it stays.  Only the visible rows are read."""
     what = "decode_window_attention"
     if q.dim() != 4 or q.shape[2] != 1:
@@ -711,6 +727,7 @@ def decode_step_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Ten
     """RoPE + append + GQA attention + slice merge of a one-token step in ONE launch (csrc/decode_step.hip): q [B,H,1,D] / k_new,
     v_new [B,Hkv,1,D] are the RAW projections, cos / sin [B,1,D] fp16; returns fp16 [B,1,H*D], the slab gains the row, len_dev is
     advanced.  `counters` + `workspace` come as a pair (new_step_counters / new_decode_workspace); nsplit 0 = the library chooses."""
+    _one_length("decode_step_attention", len_dev)
     _require_cuda(q, k_new, v_new, cos, sin, kslab, vslab, len_dev)
     B, H, one, D = q.shape
     Hkv, rows = kslab.shape[1], kslab.shape[2]

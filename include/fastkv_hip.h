@@ -372,6 +372,10 @@ int fastkv_sp_compact_f16(int32_t B, int32_t Hkv, int32_t S_r, int32_t D, int32_
  * wrote its first `capacity` rows: fastkv_update_kv_strided_f16) whose current length is an int32 in DEVICE memory: shapes
  * are static, so a whole decode step can be captured in a HIP graph and replayed.
  *   fastkv_decode_append_f16     k_new / v_new [B,Hkv,1,D] (element strides {batch, head}) -> slab row *len_dev
+ *   fastkv_decode_append         the same for fp16 or bf16 rows and, with len_step 1, one length per request: row b -> slab row
+ *                                len_dev[b] (len_step 0: len_dev[0] for all).  A negative length is an idle request: nothing is
+ *                                stored; one of `rows` or more overwrites the request's last row.  The append of
+ *                                fastkv_window_attention and fastkv_shared_prefix_attention
  *   fastkv_decode_attention_f16  q [B,H,1,D] (strides {batch, head}) attends over rows 0 .. *len_dev (the appended row
  *                                included), G = H/Hkv in {1,2,4,8} query heads share a KV head; fp32 softmax; out fp16
  *                                [B,1,H*D] contiguous; then *len_dev += 1.  nsplit = slices per KV head (8-32: the layer is
@@ -382,6 +386,9 @@ size_t fastkv_decode_workspace_bytes(int32_t B, int32_t H, int32_t D, int32_t ns
 int fastkv_decode_append_f16(int32_t B, int32_t Hkv, int32_t D, const void *k_new, const int64_t kn_strides[2], const void *v_new,
                              const int64_t vn_strides[2], void *kslab, void *vslab, const int64_t slab_strides[3], int32_t rows,
                              const int32_t *len_dev, void *stream);
+int fastkv_decode_append(int32_t B, int32_t Hkv, int32_t D, const void *k_new, const int64_t kn_strides[2], const void *v_new,
+                         const int64_t vn_strides[2], void *kslab, void *vslab, const int64_t slab_strides[3], int32_t rows,
+                         const int32_t *len_dev, int32_t len_step, void *stream);
 int fastkv_decode_attention_f16(int32_t B, int32_t H, int32_t Hkv, int32_t D, const void *q, const int64_t q_strides[2],
                                 const void *kslab, const void *vslab, const int64_t slab_strides[3], int32_t rows, int32_t *len_dev,
                                 float scaling, int32_t nsplit, void *out, void *workspace, size_t workspace_bytes, void *stream);
