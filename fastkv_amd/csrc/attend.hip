@@ -872,7 +872,7 @@ static int att_launch(AttendArgs &A, const AttPlan &P, int advance, int32_t *len
     const bool many = A.slots >= 8;
     const int per = many ? 256 / (D * 2) + (D == 256) : 1024 / D;
     const dim3 grid((unsigned)((nrows + per - 1) / per)), block(256);
-    uint32_t *flag = advance ? abort_flag_device(st) : nullptr;
+    uint32_t *flag = advance ? abort_flag_device() : nullptr;
     if (many) hipLaunchKernelGGL((attend_join_kernel<D, BF, D == 256 ? 4 : 8>), grid, block, 0, st, A, nrows, advance ? A.T : 0, len, flag);
     else hipLaunchKernelGGL((attend_join_kernel<D, BF, 1>), grid, block, 0, st, A, nrows, advance ? A.T : 0, len, flag);
     return hipGetLastError() == hipSuccess ? FASTKV_OK : FASTKV_ELAUNCH;
@@ -885,6 +885,7 @@ static int att_run(AttendArgs &A, int dtype, int D, int advance, int32_t *len, v
     const size_t need = att_bytes(P, A.B, A.H, A.T, D);
     if (need && (!workspace || ((uintptr_t)workspace & 15))) return FASTKV_EINVAL;
     if (workspace_bytes < need) return FASTKV_EWORKSPACE;
+    if (advance && !abort_flag_device()) return FASTKV_ELAUNCH;               // (no word to report a full cache in: nothing is launched that could not)
     A.G = A.H / A.Hkv;
     A.slots = P.slots;
     A.packed_tiles = P.packed_tiles;

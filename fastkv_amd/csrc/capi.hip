@@ -13,30 +13,27 @@ using namespace fk;
 // One word of pinned, host-coherent memory per process: a workgroup that gives up a hand-off wait stores 1 there.  The next
 // call of an operator entry point (or fastkv_last_status) reads and clears it on the host -- no synchronisation, no copy.
 namespace fk {
-static uint32_t *g_abort_host = nullptr, *g_abort_dev = nullptr;
-static std::once_flag g_abort_once;
+// It is allocated by the first call that needs it, whichever thread that is in, and also where a stream is being captured just then: a
+// launch recorded without the word could never report (the thread's capture mode is relaxed for the allocation, which records nothing).
+static std::atomic<uint32_t *> g_abort_host{nullptr}, g_abort_dev{nullptr};
+static std::mutex g_abort_mutex;
 uint32_t *abort_flag_device()
 {
-    std::call_once(g_abort_once, []() {
-        void *h = nullptr, *d = nullptr;
-        if (hipHostMalloc(&h, 64, hipHostMallocMapped | hipHostMallocCoherent) != hipSuccess) { (void)hipGetLastError(); return; }
-        if (hipHostGetDevicePointer(&d, h, 0) != hipSuccess) { (void)hipGetLastError(); (void)hipHostFree(h); return; }
-        reinterpret_cast<volatile uint32_t *>(h)[0] = 0;
-        reinterpret_cast<volatile uint32_t *>(h)[1] = 0;
-        reinterpret_cast<volatile uint32_t *>(h)[2] = 0;
-        reinterpret_cast<volatile uint32_t *>(h)[3] = 0;
-        reinterpret_cast<volatile uint32_t *>(h)[4] = 0;         // placement violations that are counted and never reported (mfma16 launches)
-        g_abort_host = reinterpret_cast<uint32_t *>(h);
-        g_abort_dev = reinterpret_cast<uint32_t *>(d);
-    });
-    return g_abort_dev;
-}
-uint32_t *abort_flag_device(hipStream_t st)
-{
-    if (g_abort_dev) return g_abort_dev;
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(st, &cs) != hipSuccess) (void)hipGetLastError();
-    return cs == hipStreamCaptureStatusNone ? abort_flag_device() : nullptr;
+    if (uint32_t *known = g_abort_dev.load(std::memory_order_acquire)) return known;
+    const std::lock_guard<std::mutex> lock(g_abort_mutex);
+    if (uint32_t *known = g_abort_dev.load(std::memory_order_relaxed)) return known;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+    void *h = nullptr, *d = nullptr;
+    if (hipHostMalloc(&h, 64, hipHostMallocMapped | hipHostMallocCoherent) == hipSuccess) {
+        if (hipHostGetDevicePointer(&d, h, 0) != hipSuccess) { d = nullptr; (void)hipHostFree(h); }
+    }
+    if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (!d) { (void)hipGetLastError(); return nullptr; }
+    for (int i = 0; i < 5; ++i) reinterpret_cast<volatile uint32_t *>(h)[i] = 0;     // (4: placement violations that are counted and never reported: mfma16 launches)
+    g_abort_host.store(reinterpret_cast<uint32_t *>(h), std::memory_order_release);
+    g_abort_dev.store(reinterpret_cast<uint32_t *>(d), std::memory_order_release);
+    return reinterpret_cast<uint32_t *>(d);
 }
 uint64_t spin_limit_ticks()
 {
@@ -74,22 +71,23 @@ bool no_wait_mode()
 }
 static int take_abort_status()
 {
-    if (!g_abort_host) return FASTKV_OK;
+    uint32_t *const word = g_abort_host.load(std::memory_order_acquire);
+    if (!word) return FASTKV_OK;
     // word 0: a launch gave up a bounded in-kernel wait; word 1: a decode step ran into a full cache slab (decode.hip)
     // (value 1: a bounded wait was given up -- partners that could not become resident; value 2: a workspace without a live control
     // block, a caller's error.)  Under the fail-safe policy (2, the default) a given-up wait ALSO switches the process to the no-wait
     // kernels, like a placement report does: whatever held the compute units beyond the spin limit may still be there when the caller
     // redoes the call, and a rolling launch (whose grid exceeds the chip by design) would abort again.
-    if (__atomic_load_n(g_abort_host, __ATOMIC_ACQUIRE) != 0u) {
-        const uint32_t why = __atomic_exchange_n(g_abort_host, 0u, __ATOMIC_ACQ_REL);
+    if (__atomic_load_n(word, __ATOMIC_ACQUIRE) != 0u) {
+        const uint32_t why = __atomic_exchange_n(word, 0u, __ATOMIC_ACQ_REL);
         if (why) {
             if ((why & 1u) && placement_policy().load(std::memory_order_relaxed) == 2) no_wait_flag().store(1, std::memory_order_release);
             return FASTKV_EABORTED;
         }
     }
-    if (__atomic_load_n(g_abort_host + 1, __ATOMIC_ACQUIRE) != 0u && __atomic_exchange_n(g_abort_host + 1, 0u, __ATOMIC_ACQ_REL)) return FASTKV_EOVERFLOW;
+    if (__atomic_load_n(word + 1, __ATOMIC_ACQUIRE) != 0u && __atomic_exchange_n(word + 1, 0u, __ATOMIC_ACQ_REL)) return FASTKV_EOVERFLOW;
     // word 2 (FASTKV_DEBUG_BOUNDS=1 only): a gather was handed an index outside [0, S) (compact.hip)
-    if (__atomic_load_n(g_abort_host + 2, __ATOMIC_ACQUIRE) != 0u && __atomic_exchange_n(g_abort_host + 2, 0u, __ATOMIC_ACQ_REL)) return FASTKV_EBOUNDS;
+    if (__atomic_load_n(word + 2, __ATOMIC_ACQUIRE) != 0u && __atomic_exchange_n(word + 2, 0u, __ATOMIC_ACQ_REL)) return FASTKV_EBOUNDS;
     // word 3: workgroups of a fused scoring launch that met a workgroup of ANOTHER unit on their compute unit (fused.hip: placement
     // check).  Policy (fastkv_set_placement_policy; FASTKV_STRICT_PLACEMENT at load):
     //   2 (default, "fail safe"): the launches that counted cannot vouch for their pairing -- report FASTKV_EPLACEMENT once (the caller
@@ -97,8 +95,8 @@ static int take_abort_status()
     //      is ever exposed again), so that the redo is safe whatever else runs on the GPU;
     //   1 ("strict"): report FASTKV_EPLACEMENT, change nothing;   0: count only (fastkv_placement_violations), report nothing.
     const int policy = placement_policy().load(std::memory_order_relaxed);
-    if (policy != 0 && __atomic_load_n(g_abort_host + 3, __ATOMIC_ACQUIRE) != 0u) {
-        const uint32_t n = __atomic_exchange_n(g_abort_host + 3, 0u, __ATOMIC_ACQ_REL);
+    if (policy != 0 && __atomic_load_n(word + 3, __ATOMIC_ACQUIRE) != 0u) {
+        const uint32_t n = __atomic_exchange_n(word + 3, 0u, __ATOMIC_ACQ_REL);
         if (n) {
             g_violations_reported.fetch_add(n, std::memory_order_relaxed);
             if (policy == 2) no_wait_flag().store(1, std::memory_order_release);
@@ -112,12 +110,13 @@ static int take_abort_status()
 extern "C" int fastkv_placement_violations(int reset)
 {
     (void)fk::abort_flag_device();
-    if (!fk::g_abort_host) return 0;
+    uint32_t *const word = fk::g_abort_host.load(std::memory_order_acquire);
+    if (!word) return 0;
     // pending (counted by launches, not yet reported) + already reported
-    uint64_t v = reset ? __atomic_exchange_n(fk::g_abort_host + 3, 0u, __ATOMIC_ACQ_REL) : __atomic_load_n(fk::g_abort_host + 3, __ATOMIC_ACQUIRE);
+    uint64_t v = reset ? __atomic_exchange_n(word + 3, 0u, __ATOMIC_ACQ_REL) : __atomic_load_n(word + 3, __ATOMIC_ACQUIRE);
     v += reset ? fk::g_violations_reported.exchange(0, std::memory_order_relaxed) : fk::g_violations_reported.load(std::memory_order_relaxed);
     // + what launches of the mfma16 contract counted (word 4: no policy ever acts on it)
-    v += reset ? __atomic_exchange_n(fk::g_abort_host + 4, 0u, __ATOMIC_ACQ_REL) : __atomic_load_n(fk::g_abort_host + 4, __ATOMIC_ACQUIRE);
+    v += reset ? __atomic_exchange_n(word + 4, 0u, __ATOMIC_ACQ_REL) : __atomic_load_n(word + 4, __ATOMIC_ACQUIRE);
     return (int)(v > 0x7fffffffu ? 0x7fffffffu : v);
 }
 

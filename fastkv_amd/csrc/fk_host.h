@@ -129,7 +129,6 @@ static inline Layout make_layout(const fastkv_problem &p)
 // bounded hand-off waits (fk_device.h SpinCtl): the process-wide abort flag in pinned host memory (device view; nullptr if
 // the allocation failed: the launchers then take the staged path) and the wall-clock limit in s_memrealtime ticks
 uint32_t *abort_flag_device();
-uint32_t *abort_flag_device(hipStream_t st);      // the same for a call that may be captured: nullptr where a capture would be the first to allocate it
 uint64_t spin_limit_ticks();
 bool no_wait_mode();              // FASTKV_FUSED=0 or the fail-safe switch after a placement violation (capi.hip)
 
