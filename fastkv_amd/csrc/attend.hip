@@ -847,6 +847,9 @@ static AttPlan att_plan(int B, int H, int Hkv, int D, int T, int rows, int64_t s
     return P;
 }
 
+// rows of a workgroup of the join: attend_join_kernel's ROWS
+static int att_join_rows(int slots, int D) { return slots >= 8 ? 256 / (D * 2) + (D == 256) : 1024 / D; }
+
 static size_t att_bytes(const AttPlan &P, int B, int H, int T, int D)
 {
     return (size_t)B * H * T * P.slots * (D + 2) * sizeof(float);
@@ -870,7 +873,7 @@ static int att_launch(AttendArgs &A, const AttPlan &P, int advance, int32_t *len
     const int64_t nrows = (int64_t)A.B * A.H * A.T;
     ProfScope ps_(K_ATTEND, st);
     const bool many = A.slots >= 8;
-    const int per = many ? 256 / (D * 2) + (D == 256) : 1024 / D;
+    const int per = att_join_rows(A.slots, D);
     const dim3 grid((unsigned)((nrows + per - 1) / per)), block(256);
     uint32_t *flag = advance ? abort_flag_device() : nullptr;
     if (many) hipLaunchKernelGGL((attend_join_kernel<D, BF, D == 256 ? 4 : 8>), grid, block, 0, st, A, nrows, advance ? A.T : 0, len, flag);
@@ -881,7 +884,8 @@ static int att_launch(AttendArgs &A, const AttPlan &P, int advance, int32_t *len
 static int att_run(AttendArgs &A, int dtype, int D, int advance, int32_t *len, void *workspace, size_t workspace_bytes, void *stream)
 {
     const AttPlan P = att_plan(A.B, A.H, A.Hkv, D, A.T, A.rows, (int64_t)A.window + A.sinks, A.prefix, advance != 0);
-    if (P.blocks > 0xffffff || (int64_t)A.B * A.H * A.T > 0xffffff) return FASTKV_EUNSUPPORTED;      // (a launch of less than 2^32 threads)
+    const int64_t join = P.slots ? ((int64_t)A.B * A.H * A.T + att_join_rows(P.slots, D) - 1) / att_join_rows(P.slots, D) : 0;
+    if (P.blocks > 0xffffff || join > 0xffffff) return FASTKV_EUNSUPPORTED;                          // (launches of less than 2^32 threads)
     const size_t need = att_bytes(P, A.B, A.H, A.T, D);
     if (need && (!workspace || ((uintptr_t)workspace & 15))) return FASTKV_EINVAL;
     if (workspace_bytes < need) return FASTKV_EWORKSPACE;

@@ -456,6 +456,9 @@ int fastkv_decode_gemv_f16(int32_t B, int32_t K, const void *x, int64_t x_row_st
  * one per request (len_step 1) or one for all (0); a length above rows - T counts as rows - T; NULL (window only): rows - T for all.
  * advance != 0: len_dev grows by T behind the call (not where it is negative; a full cache is reported as FASTKV_EOVERFLOW, as by
  * fastkv_decode_attention_f16).  K / V rows that nothing sees may hold anything, infinities and NaN included.  scaling > 0.
+ * Sizes: B * H * T < 2^31, rows and prefix_rows < 2^29; a call whose launches would have 2^24 workgroups or more (one per 128 rows of
+ * T * H / Hkv, or fewer rows and a slice of the keys; behind them, where there are slices or advance, one per 1 to 16 rows of B * H * T)
+ * is FASTKV_EUNSUPPORTED.
  * workspace: fastkv_attend_workspace_bytes (0: none needed; prefix 0 for the window form), 16-byte aligned, nothing to initialise and
  * nothing kept in it between calls.  Sums are added in a fixed order: the same call gives the same bits.
  */
