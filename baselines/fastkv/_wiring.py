@@ -47,11 +47,18 @@ def _static_window(config, slab):
     return win if win is not None and slab.kslab.shape[2] > win else None
 
 
-def _prefill_window(config, query_states) -> bool:
+def _window_alone(config, attention_mask, packed) -> bool:
     """FASTKV_WINDOW_ATTENTION=1: the prefill attention of a model with a sliding window runs through `ops.window_attention` instead of SDPA
-    with a dense mask (unpadded prompts, as everything here)."""
-    return os.environ.get("FASTKV_WINDOW_ATTENTION", "0") == "1" and getattr(config, "sliding_window", None) is not None \
-        and query_states.is_cuda and query_states.dtype in (torch.float16, torch.bfloat16) and query_states.shape[-1] in (64, 128, 256) \
+    with a dense mask -- where the window is all that the mask holds.  A 2-D mask that hides a token (padding: one look at its values per
+    prompt), a mask of any other form and `packed` (position ids that the mask builder may take for several sequences) stay with SDPA."""
+    if os.environ.get("FASTKV_WINDOW_ATTENTION", "0") != "1" or getattr(config, "sliding_window", None) is None or packed:
+        return False
+    return attention_mask is None or (torch.is_tensor(attention_mask) and attention_mask.dim() == 2 and bool(attention_mask.all()))
+
+
+def _prefill_window(query_states) -> bool:
+    """What `ops.window_attention` takes (see `_window_alone`)."""
+    return query_states.is_cuda and query_states.dtype in (torch.float16, torch.bfloat16) and query_states.shape[-1] in (64, 128, 256) \
         and not (torch.is_grad_enabled() and query_states.requires_grad)
 
 
@@ -160,7 +167,7 @@ def make_attention_class(base_cls, modeling, extra_attn_kwargs):
             self.tsp_idx = None
 
         def forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, fastkv_sp=None,
-                    fastkv_defer=None, **kwargs):
+                    fastkv_defer=None, fastkv_window=False, **kwargs):
             input_shape = hidden_states.shape[:-1]
             hidden_shape = (*input_shape, -1, self.head_dim)
             q_len = input_shape[1]
@@ -230,7 +237,7 @@ def make_attention_class(base_cls, modeling, extra_attn_kwargs):
                         return self.o_proj(attn_output.view(*input_shape, -1)), None
                     key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)
 
-            if q_len > 1 and key_states.shape[2] == q_len and not self.training and _prefill_window(self.config, query_states):
+            if fastkv_window and q_len > 1 and key_states.shape[2] == q_len and not self.training and _prefill_window(query_states):
                 attn_output = ops.window_attention(query_states, key_states, value_states, window=self.config.sliding_window, scaling=self.scaling)
                 return self.o_proj(attn_output), None
 
@@ -305,7 +312,7 @@ def make_attention_class(base_cls, modeling, extra_attn_kwargs):
 
 
 def decoderlayer_forward_fastkv(self, hidden_states, attention_mask=None, position_ids=None, past_key_values=None,
-                                use_cache=False, position_embeddings=None, fastkv_sp=None, fastkv_defer=None, **kwargs):
+                                use_cache=False, position_embeddings=None, fastkv_sp=None, fastkv_defer=None, fastkv_window=False, **kwargs):
     static = _static_step(past_key_values, hidden_states)
     if static and fastkv_sp is None and _static_layer_ok(self, hidden_states, position_embeddings, past_key_values):
         return _static_layer(self, hidden_states, position_embeddings, past_key_values)
@@ -313,7 +320,8 @@ def decoderlayer_forward_fastkv(self, hidden_states, attention_mask=None, positi
     hidden_states = _norm(self.input_layernorm, hidden_states, static)
     hidden_states, _ = self.self_attn(hidden_states=hidden_states, attention_mask=attention_mask, position_ids=position_ids,
                                       past_key_values=past_key_values, use_cache=use_cache,
-                                      position_embeddings=position_embeddings, fastkv_sp=fastkv_sp, fastkv_defer=fastkv_defer, **kwargs)
+                                      position_embeddings=position_embeddings, fastkv_sp=fastkv_sp, fastkv_defer=fastkv_defer,
+                                      fastkv_window=fastkv_window, **kwargs)
     hidden_states = residual + hidden_states
     residual = hidden_states
     hidden_states = _norm(self.post_attention_layernorm, hidden_states, static)
@@ -382,6 +390,7 @@ def make_model_forward(modeling, mask_fn_for):
             inputs_embeds = self.embed_tokens(input_ids)
         if use_cache and past_key_values is None:
             past_key_values = make_cache(self.config)
+        packed = position_ids is not None and past_key_values is None
         sp = getattr(self, "_fastkv_sp", None)                    # sequence-parallel prefill (fastkv_amd/sp_model.py)
         if sp is not None and position_ids is None:
             position_ids = (torch.arange(inputs_embeds.shape[1], device=inputs_embeds.device) + sp.pos0).unsqueeze(0)
@@ -400,6 +409,7 @@ def make_model_forward(modeling, mask_fn_for):
         else:
             causal_mask = mask_fn_for(self.config)(config=self.config, inputs_embeds=inputs_embeds, attention_mask=attention_mask,
                                                    past_key_values=past_key_values, position_ids=position_ids)
+        window_alone = sp is None and inputs_embeds.shape[1] > 1 and _window_alone(self.config, attention_mask, packed)
         hidden_states = inputs_embeds
         position_embeddings = _step_rotary(self.rotary_emb, hidden_states, position_ids, past_key_values)
         # Prefill: layers whose compressed cache is not needed while the prompt is in flight (all but the TSP layer) are compressed
@@ -418,7 +428,8 @@ def make_model_forward(modeling, mask_fn_for):
         for decoder_layer in self.layers[: self.config.num_hidden_layers]:
             hidden_states = decoder_layer(hidden_states, attention_mask=causal_mask, position_embeddings=position_embeddings,
                                           position_ids=position_ids, past_key_values=past_key_values, use_cache=use_cache,
-                                          fastkv_sp=sp if (sp is not None and not sp.reduced) else None, fastkv_defer=defer, **kwargs)
+                                          fastkv_sp=sp if (sp is not None and not sp.reduced) else None, fastkv_defer=defer,
+                                          fastkv_window=window_alone, **kwargs)
             new_position_ids = getattr(decoder_layer, "new_position_ids", None)
             if new_position_ids is not None:                      # after the TSP layer: fewer tokens, new rotary tables
                 position_ids = new_position_ids
@@ -430,6 +441,7 @@ def make_model_forward(modeling, mask_fn_for):
                 # over the current K/V), and no position ids: the gaps between surviving positions are not sequence boundaries.
                 causal_mask = mask_fn_for(self.config)(config=self.config, inputs_embeds=hidden_states, attention_mask=None,
                                                        past_key_values=None, position_ids=None)
+                window_alone = sp is None and _window_alone(self.config, None, False)
         if defer is not None:
             for idx, k_c, v_c in defer.flush():                   # (layer order: the cache grows by appending)
                 past_key_values.update(k_c, v_c, idx)
