@@ -56,10 +56,11 @@ def _window_alone(config, attention_mask, packed) -> bool:
     return attention_mask is None or (torch.is_tensor(attention_mask) and attention_mask.dim() == 2 and bool(attention_mask.all()))
 
 
-def _prefill_window(query_states) -> bool:
-    """What `ops.window_attention` takes (see `_window_alone`)."""
-    return query_states.is_cuda and query_states.dtype in (torch.float16, torch.bfloat16) and query_states.shape[-1] in (64, 128, 256) \
-        and not (torch.is_grad_enabled() and query_states.requires_grad)
+def _prefill_window(*states) -> bool:
+    """What `ops.window_attention` takes (see `_window_alone`); a gradient of any of q, k, v needs SDPA, whichever projections are trained."""
+    q = states[0]
+    return q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and q.shape[-1] in (64, 128, 256) \
+        and not (torch.is_grad_enabled() and any(t.requires_grad for t in states))
 
 
 def _norm(module, hidden_states, static):
@@ -237,7 +238,8 @@ def make_attention_class(base_cls, modeling, extra_attn_kwargs):
                         return self.o_proj(attn_output.view(*input_shape, -1)), None
                     key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)
 
-            if fastkv_window and q_len > 1 and key_states.shape[2] == q_len and not self.training and _prefill_window(query_states):
+            if fastkv_window and q_len > 1 and key_states.shape[2] == q_len and not self.training \
+                    and _prefill_window(query_states, key_states, value_states):
                 attn_output = ops.window_attention(query_states, key_states, value_states, window=self.config.sliding_window, scaling=self.scaling)
                 return self.o_proj(attn_output), None
 

@@ -19,3 +19,12 @@ def test_only_a_window_alone(monkeypatch, mask, packed, takes):
     assert _wiring._window_alone(config, mask, packed) is takes
     assert not _wiring._window_alone(types.SimpleNamespace(sliding_window=None), mask, packed)
     assert not _wiring._window_alone(types.SimpleNamespace(), mask, packed)
+
+
+@pytest.mark.parametrize("trained", ["q", "k", "v", None])
+def test_a_gradient_of_any_projection_keeps_sdpa(trained):
+    """An adapter on the key or value projection alone: the kernel has no backward pass, and refuses."""
+    states = [types.SimpleNamespace(is_cuda=True, dtype=torch.float16, shape=(1, 4, 9, 64), requires_grad=n == trained) for n in "qkv"]
+    assert _wiring._prefill_window(*states) is (trained is None)
+    with torch.no_grad():
+        assert _wiring._prefill_window(*states)
