@@ -32,12 +32,26 @@ def _window_allows_static(config, past_key_values) -> bool:
     """The HIP decode attention attends over ALL rows of the slab (no mask: one new token sees the whole cache).  A model with a
     sliding window (Mistral v0.1: `config.sliding_window`) limits attention to the last `window` positions in the eager path
     (mistral_model.py passes the window to the mask builder and the attention call): the two agree only while the slabs cannot
-    hold more rows than the window.  Otherwise the step's attention is `ops.decode_window_attention` (see `_static_window`)."""
+    hold more rows than the window.  Otherwise the step's attention is `ops.decode_window_attention` (see `_static_window`), where that
+    takes the slabs."""
     win = getattr(config, "sliding_window", None)
     if win is None:
         return True
     layers = getattr(past_key_values, "layers", None) or []
     return all(getattr(l, "kslab", None) is None or l.kslab.shape[2] <= win for l in layers)
+
+
+def _require_window_decode(config, past_key_values) -> None:
+    """Refuses a static step up front -- before its first layer has written a row -- where its slabs outgrow the window and
+    `ops.decode_window_attention` does not take them."""
+    if _window_allows_static(config, past_key_values):
+        return
+    for l in past_key_values.layers:
+        s = getattr(l, "kslab", None)
+        if s is not None and (s.dtype not in (torch.float16, torch.bfloat16) or s.shape[3] not in (64, 128, 256)):
+            raise ValueError(f"static decode of a model with sliding_window = {config.sliding_window} and slabs of more rows needs fp16 or bf16 and a "
+                             f"head_dim of 64, 128 or 256, got {s.dtype}, {s.shape[3]}: decode eagerly (cache.finish_static_decode()) or size the "
+                             "slabs within the window")
 
 
 def _static_window(config, slab):
@@ -397,6 +411,8 @@ def make_model_forward(modeling, mask_fn_for):
         if sp is not None and position_ids is None:
             position_ids = (torch.arange(inputs_embeds.shape[1], device=inputs_embeds.device) + sp.pos0).unsqueeze(0)
             position_ids = position_ids.expand(inputs_embeds.shape[0], -1)
+        if getattr(past_key_values, "static_decode", False):
+            _require_window_decode(self.config, past_key_values)
         if position_ids is None:
             if getattr(past_key_values, "static_decode", False):
                 raise ValueError("static decode (graph-capturable) needs position_ids as a device tensor: a host-side position "
