@@ -916,6 +916,8 @@ static bool att_shape_ok(int dtype, int B, int H, int Hkv, int D, int T, int row
     return (dtype == FASTKV_F16 || dtype == FASTKV_BF16) && B >= 1 && Hkv >= 1 && H >= Hkv && H % Hkv == 0 && T >= 1 && rows >= 1 &&
            (int64_t)B * H * T <= 0x7fffffff && rows <= 0x1fffffff && D >= 1;
 }
+// (scores are taken times scaling * log2(e), which has to be a number too)
+static bool att_scaling_ok(float scaling) { return scaling > 0.0f && scaling * 1.44269504088896340736f < INFINITY; }
 // 16-byte rows of [n0,n1,n2] or [n1,n2]; along an extent of one nothing is stepped, whatever stride the caller has for it: it becomes 0 in `to`
 static bool att_rows_ok(const void *p, const int64_t *s, std::initializer_list<int> extents, std::initializer_list<int64_t *> to)
 {
@@ -954,7 +956,7 @@ int fastkv_window_attention(int32_t dtype, int32_t B, int32_t H, int32_t Hkv, in
     if (!att_rows_ok(q, q_strides, {B, H, T}, {&A.q_b, &A.q_h, &A.q_t}) || !att_rows_ok(k, k_strides, {B, Hkv, rows}, {&A.k_b, &A.k_h, &A.k_r}) ||
         !att_rows_ok(v, v_strides, {B, Hkv, rows}, {&A.v_b, &A.v_h, &A.v_r}) || !out || ((uintptr_t)out & 15))
         return FASTKV_EINVAL;
-    if (window < 0 || sinks < 0 || !(scaling > 0.0f) || scaling > 3.0e38f || len_step < 0 || len_step > 1 || (advance && !len_dev)) return FASTKV_EINVAL;
+    if (window < 0 || sinks < 0 || !att_scaling_ok(scaling) || len_step < 0 || len_step > 1 || (advance && !len_dev)) return FASTKV_EINVAL;
     A.q = (const uint16_t *)q;
     A.k = A.k0 = (const uint16_t *)k;
     A.k0_b = A.k_b; A.k0_h = A.k_h; A.k0_r = A.k_r;
@@ -985,7 +987,7 @@ int fastkv_shared_prefix_attention(int32_t dtype, int32_t B, int32_t H, int32_t 
         !att_rows_ok(k_prefix, kp_strides, {Hkv, prefix_rows}, {&A.k0_h, &A.k0_r}) ||
         !att_rows_ok(v_prefix, vp_strides, {Hkv, prefix_rows}, {&A.v0_h, &A.v0_r}) || !out || ((uintptr_t)out & 15))
         return FASTKV_EINVAL;
-    if (!(scaling > 0.0f) || scaling > 3.0e38f || !len_dev || len_step < 0 || len_step > 1) return FASTKV_EINVAL;
+    if (!att_scaling_ok(scaling) || !len_dev || len_step < 0 || len_step > 1) return FASTKV_EINVAL;
     A.q = (const uint16_t *)q;
     A.k0 = (const uint16_t *)k_prefix;
     A.v0 = (const uint16_t *)v_prefix;

@@ -455,7 +455,8 @@ int fastkv_decode_gemv_f16(int32_t B, int32_t K, const void *x, int64_t x_row_st
  * all multiples of 8 (along an extent of one: any), head-dim stride 1, 16-byte aligned bases.  rows: rows of the cache per request.  len_dev: int32 on the device,
  * one per request (len_step 1) or one for all (0); a length above rows - T counts as rows - T; NULL (window only): rows - T for all.
  * advance != 0: len_dev grows by T behind the call (not where it is negative; a full cache is reported as FASTKV_EOVERFLOW, as by
- * fastkv_decode_attention_f16).  K / V rows that nothing sees may hold anything, infinities and NaN included.  scaling > 0.
+ * fastkv_decode_attention_f16).  K / V rows that nothing sees may hold anything, infinities and NaN included.  scaling > 0, and
+ * scaling * log2(e) finite.
  * Sizes: B * H * T < 2^31, rows and prefix_rows < 2^29; a call whose launches would have 2^24 workgroups or more (one per 128 rows of
  * T * H / Hkv, or fewer rows and a slice of the keys; behind them, where there are slices or advance, one per 1 to 16 rows of B * H * T)
  * is FASTKV_EUNSUPPORTED.
