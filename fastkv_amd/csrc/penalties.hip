@@ -132,6 +132,17 @@ template <int DT> static void pen_launch(const PenaltyArgs &A, int B, bool vec, 
     else hipLaunchKernelGGL((penalties_kernel<DT, false>), grid, dim3(PEN_THREADS), lds, st, A);
 }
 
+// Rows of aw bytes, as apart, na of them from `a` on, and such rows from `b` on: no byte is in both.  (Equal distances: also where the rows lie between
+// each other, like two halves of one wide tensor.)
+static bool pen_apart(uintptr_t a, int64_t na, int64_t as, int64_t aw, uintptr_t b, int64_t nb, int64_t bs, int64_t bw)
+{
+    const uintptr_t a1 = a + (na - 1) * as + aw, b1 = b + (nb - 1) * bs + bw;
+    if (a1 <= b || b1 <= a) return true;
+    if (as != bs || as <= 0) return false;
+    const int64_t d = b >= a ? (int64_t)((b - a) % as) : (as - (int64_t)((a - b) % as)) % as;
+    return d >= aw && d + bw <= as;
+}
+
 }  // namespace fk
 
 using namespace fk;
@@ -148,11 +159,18 @@ extern "C" int fastkv_decode_penalties(int32_t dtype, int32_t B, int32_t V, cons
     if ((L > 0 && (!tokens || token_stride < 0)) || bias_stride < 0 || allowed_stride < 0) return FASTKV_EINVAL;
     const int word = dtype == FASTKV_F32 ? 4 : 2;
     if (((uintptr_t)logits | (uintptr_t)out) % word || ((uintptr_t)tokens & 7)) return FASTKV_EINVAL;
-    const uintptr_t a0 = (uintptr_t)logits, a1 = a0 + ((size_t)(B - 1) * row_stride + V) * word;
-    const uintptr_t o0 = (uintptr_t)out, o1 = o0 + ((size_t)(B - 1) * out_stride + V) * word;
-    if (a0 < o1 && o0 < a1 && !(a0 == o0 && (row_stride == out_stride || B == 1))) return FASTKV_EINVAL;      // in place, or apart
     const int32_t steps[5] = {n_tokens_step, n_prompt_step, repetition_step, presence_step, frequency_step};
     for (int i = 0; i < 5; ++i) if (steps[i] < 0 || steps[i] > 1) return FASTKV_EINVAL;
+    // in place, or apart; and what other workgroups still read is never written
+    auto out_apart = [&](const void *p, int64_t n, int64_t stride, int64_t width) {
+        return !p || pen_apart((uintptr_t)out, B, out_stride * word, (int64_t)V * word, (uintptr_t)p, n, stride, width);
+    };
+    if (!(logits == out && (row_stride == out_stride || B == 1)) && !out_apart(logits, B, row_stride * word, (int64_t)V * word)) return FASTKV_EINVAL;
+    if ((L > 0 && !out_apart(tokens, B, token_stride * 8, (int64_t)L * 8)) || !out_apart(bias, B, bias_stride * 4, (int64_t)V * 4) ||
+        !out_apart(allowed, B, allowed_stride * 4, (V + 31LL) / 32 * 4))
+        return FASTKV_EINVAL;
+    const void *const values[5] = {n_tokens, n_prompt, repetition, presence, frequency};
+    for (int i = 0; i < 5; ++i) if (!out_apart(values[i], B, steps[i] * 4, 4)) return FASTKV_EINVAL;
     PenaltyArgs A = {};
     A.logits = logits;
     A.out = out;

@@ -645,7 +645,7 @@ def decode_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None
     `bias` is added; a token whose bit v % 32 of word v // 32 of `allowed` is clear becomes -inf.
     tokens int64 [B,L] (ids outside [0,V) count for nothing); n_tokens, n_prompt int32 [B] or [1] (None: L, 0); repetition (> 0), presence,
     frequency fp32 [B] or [1]; bias fp32 [V], [1,V] or [B,V]; allowed int32 [words], [1,words] or [B,words], words = ceil(V/32); all on the
-    device.  `out`: where the result goes (`logits` itself: in place); a new tensor if None."""
+    device.  `out`: where the result goes (`logits` itself: in place; no other argument's memory); a new tensor if None."""
     what = "decode_penalties"
     code = _LOGITS_DTYPE.get(logits.dtype)
     if code is None or logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):

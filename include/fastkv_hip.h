@@ -483,7 +483,8 @@ int fastkv_shared_prefix_attention(int32_t dtype, int32_t B, int32_t H, int32_t 
  *   x += bias[b, v];  bit v % 32 of allowed[b, v / 32] clear: x = -inf
  * tokens int64 [B,L] (ids outside [0,V) count for nothing), n_tokens / n_prompt int32, the three penalties fp32, all on the device;
  * `*_step` 1: one value per row, 0: one for all; NULL: L / 0 / that penalty is not applied.  bias fp32, allowed uint32 words: row
- * stride 0 = one row for all, NULL: none.  Strides in elements.  out may be `logits` itself with the same stride, and may not overlap it otherwise.
+ * stride 0 = one row for all, NULL: none.  Strides in elements.  out may be `logits` itself with the same stride; otherwise no
+ * element of it may be one of `logits` or of another argument (rows of one stride may lie between each other).
  */
 int fastkv_decode_penalties(int32_t dtype, int32_t B, int32_t V, const void *logits, int64_t row_stride, const int64_t *tokens,
                             int64_t token_stride, int32_t L, const int32_t *n_tokens, int32_t n_tokens_step, const int32_t *n_prompt,
