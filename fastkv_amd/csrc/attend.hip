@@ -26,15 +26,15 @@
 // Tiles go from memory to shared memory without passing registers (a wave has 512 / 2 of them at 128 dims, all in use).
 // Work too small to fill the chip is cut along the keys; slices leave {m, l, O} in a workspace and attend_join adds them up.
 //
-// What bounds it, measured (H 32, Hkv 8, D 128):
-//   prompts   the matrix pipe, the vector pipe and the clock together: 8k tokens, window 4096: 0.43 ms, 960 TFLOP/s (an 8192^3 library product:
-//             1110); 32k: 2.12 ms, 970.  Per tile of a wave 1024 cycles of products beside ~1000 of vector work; the clock falls to
+// What bounds it, measured (H 32, Hkv 8, D 128; times in the kernels, medians of 36 calls on one card -- another card was 3 % faster on the prompts):
+//   prompts   the matrix pipe, the vector pipe and the clock together: 8k tokens, window 4096: 0.448 ms, 920 TFLOP/s (an 8192^3 library product:
+//             1110); 32k: 2.18 ms, 948.  Per tile of a wave 1024 cycles of products beside ~1000 of vector work; the clock falls to
 //             1.95 GHz under it.  Leaving out the exponentials / the loads / the second product gives 7 / 14 / 12 %: nothing alone bounds it.
 //             Slower: two groups of waves held half a tile apart by barriers (0.53 ms), raised wave priorities (+3 %), exponentials
 //             interleaved with products by hand (+3 %), 32-key tiles (registers spill at three waves per SIMD).
 //   tokens    the memory: 32 requests, window 4096: 88 us, 5.4 TB/s of K and V (a large copy: 5.1 read + write); one request, window 2048:
-//             7.3 + 3.9 us, the latency of the chain kernel arguments - length - K - V - join - second launch
-//   prefix    64 requests on 32768 shared rows: 65 + 9 us: 38 of products (twice 128 rows per KV head), 13 of the requests' own rows, the
+//             8.1 + 3.9 us, the latency of the chain kernel arguments - length - K - V - join - second launch
+//   prefix    64 requests on 32768 shared rows: 66 + 9 us: 38 of products (twice 128 rows per KV head), 13 of the requests' own rows, the
 //             slices' sums.  Alternating the shared and the own items over the grid is slower (84): a lone rows-shaped workgroup on a compute unit
 //             has nothing beside its products.
 #include <limits.h>

@@ -6,7 +6,7 @@
 // Bound by the bytes of the logits (read and written once).  A workgroup owns a run of the vocabulary: it walks the row's whole history,
 // counts the ids that fall into its run in shared memory (integer additions: no order to depend on) and then streams its logits through.
 // The history is read once per run and row, out of L2; the alternative, a table of counts per row in memory, costs 4 bytes per
-// vocabulary entry each step instead.  Measured: 64 rows of 131072 fp32 logits with biases and masks per row 20.9 us (103 MB: 4.9 TB/s; a
+// vocabulary entry each step instead.  Measured (medians): 64 rows of 131072 fp32 logits with biases and masks per row 20.8 us (103 MB: 4.9 TB/s; a
 // large copy 5.1); one row of 128256 fp16 logits with a history of 2304: 5.0 us, a launch's latency and two passes through shared memory.
 #include "fk_device.h"
 #include "fk_host.h"

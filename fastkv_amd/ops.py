@@ -601,8 +601,10 @@ def decode_shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_pr
                                    len_dev: torch.Tensor, scaling: float, advance: bool = True) -> torch.Tensor:
     """Attention of a batch that continues ONE prefix (a compressed document, many questions): q [B,H,T,D], T >= 1; k_prefix, v_prefix
     [Hkv,P,D] or [1,Hkv,P,D]; kslab, vslab [B,Hkv,rows,D] the requests' own rows -> [B,T,H*D].  Every query sees the whole prefix and its
-    request's own rows j <= len_dev[b] + t (the T new rows are already written there); the prefix is read once for the batch.
-    len_dev (int32 [1] or [B]) moves on by T on the device unless `advance` is False; len_dev[b] + t < 0 is idle: zeros."""
+    request's own rows j <= len_dev[b] + t (the T new rows are already written there).  With T * H / Hkv < 128 rows per request the prefix is
+    read once for the batch; the tiles of longer questions are one request's each.
+    len_dev (int32 [1] or [B]) moves on by T on the device unless `advance` is False; len_dev[b] + t < 0 is idle: zeros.  A negative length
+    stays as it is, also where some of the T tokens are in use (a question padded at the left): its next length, len + T, is the caller's."""
     what = "decode_shared_prefix_attention"
     if len_dev is None or k_prefix is None or v_prefix is None:
         raise ValueError(f"fastkv_amd.{what}: a prefix and len_dev expected")

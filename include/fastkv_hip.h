@@ -450,11 +450,12 @@ int fastkv_decode_gemv_f16(int32_t B, int32_t K, const void *x, int64_t x_row_st
  * type = sum softmax(scaling q.k) v over the rows it sees, fp32 sums; p < 0 (an idle request, left padding): zeros.
  *   fastkv_window_attention          rows j <= p of the request's cache with j < sinks or j > p - window (window 0: all j <= p)
  *   fastkv_shared_prefix_attention   all prefix_rows rows of ONE prefix [Hkv,prefix_rows,D] that every request continues, and the
- *                                    request's own rows j <= p.  The prefix is read once for the batch, not once per request
+ *                                    request's own rows j <= p.  With T * H / Hkv < 128 rows per request the prefix is read once for the
+ *                                    batch; the tiles of longer questions are one request's each and read it from the caches
  * dtype FASTKV_F16 | FASTKV_BF16; D 64, 128 or 256; element strides q {batch, head, token}, k / v {batch, head, row}, prefix {head, row}:
  * all multiples of 8 (along an extent of one: any), head-dim stride 1, 16-byte aligned bases.  rows: rows of the cache per request.  len_dev: int32 on the device,
  * one per request (len_step 1) or one for all (0); a length above rows - T counts as rows - T; NULL (window only): rows - T for all.
- * advance != 0: len_dev grows by T behind the call (not where it is negative; a full cache is reported as FASTKV_EOVERFLOW, as by
+ * advance != 0: len_dev grows by T behind the call (not where it is negative, which a left-padded request's is too; a full cache is reported as FASTKV_EOVERFLOW, as by
  * fastkv_decode_attention_f16).  K / V rows that nothing sees may hold anything, infinities and NaN included.  scaling > 0, and
  * scaling * log2(e) finite.
  * Sizes: B * H * T < 2^31, rows and prefix_rows < 2^29; a call whose launches would have 2^24 workgroups or more (one per 128 rows of
