@@ -576,7 +576,7 @@ def _window_of(what, window, sinks):
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
                      scaling: Optional[float] = None, len_dev: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of T queries per request with a sliding window and sinks (csrc/attend.hip): q [B,H,T,D], k, v [B,Hkv,rows,D] fp16 or
-    bf16 (any strides, unit head_dim stride) -> [B,T,H*D].  Query t of request b stands at p = len_dev[b] + t and sees the rows j <= p
+    bf16 (unit head_dim stride, the others multiples of 8; 16-byte aligned) -> [B,T,H*D].  Query t of request b stands at p = len_dev[b] + t and sees the rows j <= p
     with j < sinks or j > p - window; `window` None: all j <= p.  `len_dev` (int32 [B] or [1], on the device): rows in front of the T
     new ones, whose K / V are already in rows len .. len+T-1; None: the last T of all rows.  p < 0 (left padding): zeros."""
     window, sinks = _window_of("window_attention", window, sinks)

@@ -461,7 +461,8 @@ int fastkv_decode_gemv_f16(int32_t B, int32_t K, const void *x, int64_t x_row_st
  * Sizes: B * H * T < 2^31, rows and prefix_rows < 2^29; a call whose launches would have 2^24 workgroups or more (one per 128 rows of
  * T * H / Hkv, or fewer rows and a slice of the keys; behind them, where there are slices or advance, one per 1 to 16 rows of B * H * T)
  * is FASTKV_EUNSUPPORTED.
- * workspace: fastkv_attend_workspace_bytes (0: none needed; prefix 0 for the window form), 16-byte aligned, nothing to initialise and
+ * workspace: fastkv_attend_workspace_bytes (0: none needed; prefix 0 for the window form, window and sinks 0
+ * for the other), 16-byte aligned, nothing to initialise and
  * nothing kept in it between calls.  Sums are added in a fixed order: the same call gives the same bits.
  */
 size_t fastkv_attend_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t T, int32_t rows, int32_t window, int32_t sinks,
